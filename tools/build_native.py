@@ -49,6 +49,9 @@ EXTENSIONS = {
     "contrib": ("contrib.cpp", ("comm", "pool", "transducer", "transformer")),
 }
 CORE_DIRS = ("mta",)
+# hipcc -O3 forms v_pk_{add,mul,fma}_f32 from ordinary float code; some of their operand forms have
+# given wrong results on MI355X, so device code is compiled without the packed-fp32 instructions
+NO_PACKED_FP32 = ("-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops")
 
 # binding file -> macro that module.cpp keys on
 SUBSYSTEMS = {
@@ -162,7 +165,7 @@ def compile_cmds(verbose: bool, extensions=None, out=None, build_dir=BUILD, defi
     common = ["-std=c++17", "-O3", "-fPIC", f"-I{os.path.join(CSRC, 'include')}", "-Wno-unused-result",
               "-Wno-deprecated-declarations", "-Wno-unused-command-line-argument", *[f"-D{d}" for d in defines]]
     dev = [HIPCC, *common, f"--offload-arch={ARCH}", "-munsafe-fp-atomics", "-ffp-contract=fast",
-           "--no-offload-compress", "-x", "hip"]
+           "--no-offload-compress", *NO_PACKED_FP32, "-x", "hip"]
     host = [HIPCC, *common, "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_C",
             "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *macros,
             *[f"-isystem{p}" for p in tinc], f"-isystem{py_inc}", "-fvisibility=hidden"]
