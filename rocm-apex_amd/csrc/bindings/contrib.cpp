@@ -4,6 +4,7 @@
 #include "common.h"
 #include "apex_amd/transducer_api.h"
 #include "apex_amd/pool_api.h"
+#include "apex_amd/qk_norm_rope_api.h"
 
 namespace apex_amd {
 
@@ -22,6 +23,8 @@ void peer_allgather(const float* local, int n, int nmax, float* const* bufs, int
                     float* out, int* err, double timeout_s, hipStream_t s);
 
 namespace {
+
+bool has_tensor(const c10::optional<at::Tensor>& t) { return t.has_value() && t->defined(); }
 
 // ---- peer memory (hipIpc over xGMI) exchange: csrc/comm/peer.hip ----
 pybind11::tuple pm_alloc(int64_t bytes) {
@@ -83,6 +86,120 @@ at::Tensor bda_backward(const at::Tensor& g, double p, int64_t seed, int64_t off
   bias_dropout_add_bwd(gc.data_ptr(), dx.data_ptr(), gc.numel(), dtype_code(g.scalar_type()), (float)p, (uint64_t)seed,
                        (uint64_t)offset, device_cus(g.get_device()), cur_stream(), step_ptr(rng_step));
   return dx;
+}
+
+// ---- per-head RMS norm + rotary rotation of q and k (csrc/transformer/qk_norm_rope.hip) ----
+// Everything the kernels index with is checked here: [a, b, heads, d] operands on one device, d
+// contiguous, tables [table, rot / 2], positions of (or broadcast to) the token axes.
+struct QkRopeHold {
+  QkRopeArgs a{};
+  at::Tensor pos, cos, sin, qw, kw;
+};
+
+QkRopeView qk_view(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+
+void qk_check4(const at::Tensor& t, const at::Tensor& like, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.get_device() == like.get_device() && t.scalar_type() == like.scalar_type() &&
+                  t.dim() == 4 && t.size(0) == like.size(0) && t.size(1) == like.size(1) &&
+                  t.size(3) == like.size(3) && (t.stride(3) == 1 || t.size(3) == 1),
+              "qk_norm_rope: ", what, " must be a [a, b, heads, d] tensor of q's dtype and device, d contiguous");
+}
+
+void qk_setup(QkRopeHold& h, const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& qw,
+              const c10::optional<at::Tensor>& kw, const at::Tensor& cos, const at::Tensor& sin,
+              const at::Tensor& positions, double eps, bool interleaved) {
+  qk_check4(q, q, "q");
+  qk_check4(k, q, "k");
+  const int64_t d = q.size(3);
+  TORCH_CHECK(d >= 2 && d % 2 == 0 && d <= kQkRopeMaxDim, "qk_norm_rope: head size must be even and <= ", kQkRopeMaxDim);
+  TORCH_CHECK(q.size(2) < (1 << 20) && k.size(2) < (1 << 20), "qk_norm_rope: too many heads");
+  auto on_dev = [&](const at::Tensor& t) { return t.is_cuda() && t.get_device() == q.get_device(); };
+  TORCH_CHECK(on_dev(cos) && on_dev(sin) && cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat &&
+                  cos.dim() == 2 && cos.sizes() == sin.sizes() && 2 * cos.size(1) <= d,
+              "qk_norm_rope: cos and sin must be fp32 [positions, rot / 2] tables on q's device, rot <= head size");
+  TORCH_CHECK(on_dev(positions) && positions.dim() == 2 && positions.size(0) == q.size(0) &&
+                  positions.size(1) == q.size(1) &&
+                  (positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt),
+              "qk_norm_rope: positions must be an integer [a, b] tensor on q's device");
+  TORCH_CHECK(has_tensor(qw) == has_tensor(kw), "qk_norm_rope: give both norm weights or neither");
+  QkRopeArgs& a = h.a;
+  a.n0 = q.size(0);
+  a.n1 = q.size(1);
+  a.hq = (int)q.size(2);
+  a.hk = (int)k.size(2);
+  a.d = (int)d;
+  a.rot = 2 * (int)cos.size(1);
+  a.q = qk_view(q);
+  a.k = qk_view(k);
+  h.cos = cos.contiguous();
+  h.sin = sin.contiguous();
+  h.pos = positions.to(at::kLong);
+  a.cos = h.cos.data_ptr<float>();
+  a.sin = h.sin.data_ptr<float>();
+  a.table = cos.size(0);
+  TORCH_CHECK(a.table > 0 || q.numel() + k.numel() == 0, "qk_norm_rope: empty tables");
+  a.pos = h.pos.data_ptr<int64_t>();
+  a.ps0 = h.pos.stride(0);
+  a.ps1 = h.pos.stride(1);
+  a.eps = (float)eps;
+  a.interleaved = interleaved;
+  a.dtype = dtype_code(q.scalar_type());
+  if (has_tensor(qw)) {
+    for (const auto* w : {&*qw, &*kw})
+      TORCH_CHECK(on_dev(*w) && w->numel() == d && w->scalar_type() == qw->scalar_type() &&
+                      (w->scalar_type() == at::kFloat || w->scalar_type() == q.scalar_type()),
+                  "qk_norm_rope: norm weights must be [d], both fp32 or both of q's dtype, on q's device");
+    h.qw = qw->contiguous();
+    h.kw = kw->contiguous();
+    a.qw = h.qw.data_ptr();
+    a.kw = h.kw.data_ptr();
+    a.wdtype = dtype_code(h.qw.scalar_type());
+  }
+}
+
+std::vector<at::Tensor> qk_forward(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& qw,
+                                   const c10::optional<at::Tensor>& kw, const at::Tensor& cos, const at::Tensor& sin,
+                                   const at::Tensor& positions, double eps, bool interleaved) {
+  TORCH_CHECK(q.is_cuda(), "qk_norm_rope: GPU tensors expected");
+  const c10::hip::HIPGuard guard(q.get_device());
+  QkRopeHold h;
+  qk_setup(h, q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  h.a.qo = qk_view(qo);
+  h.a.ko = qk_view(ko);
+  qk_norm_rope_fwd(h.a, device_cus(q.get_device()), cur_stream());
+  return {qo, ko};
+}
+
+std::vector<at::Tensor> qk_backward(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q,
+                                    const at::Tensor& k, const c10::optional<at::Tensor>& qw,
+                                    const c10::optional<at::Tensor>& kw, const at::Tensor& cos, const at::Tensor& sin,
+                                    const at::Tensor& positions, double eps, bool interleaved) {
+  TORCH_CHECK(q.is_cuda(), "qk_norm_rope: GPU tensors expected");
+  const c10::hip::HIPGuard guard(q.get_device());
+  QkRopeHold h;
+  qk_setup(h, q, k, qw, kw, cos, sin, positions, eps, interleaved);
+  qk_check4(gq, q, "the gradient of q");
+  qk_check4(gk, q, "the gradient of k");
+  TORCH_CHECK(gq.size(2) == q.size(2) && gk.size(2) == k.size(2), "qk_norm_rope: gradient shape mismatch");
+  at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
+  h.a.gq = qk_view(gq);
+  h.a.gk = qk_view(gk);
+  h.a.qo = qk_view(dq);
+  h.a.ko = qk_view(dk);
+  at::Tensor dqw, dkw, part;
+  const int cus = device_cus(q.get_device());
+  if (h.a.qw != nullptr) {
+    const bool empty = q.size(0) * q.size(1) == 0 || q.size(2) + k.size(2) == 0;
+    dqw = empty ? at::zeros({q.size(3)}, h.qw.options()) : at::empty({q.size(3)}, h.qw.options());
+    dkw = empty ? at::zeros({q.size(3)}, h.qw.options()) : at::empty({q.size(3)}, h.qw.options());
+    part = at::empty({qk_norm_rope_part_floats(h.a, cus)}, q.options().dtype(at::kFloat));
+    h.a.part = part.data_ptr<float>();
+    h.a.dqw = dqw.data_ptr();
+    h.a.dkw = dkw.data_ptr();
+  }
+  qk_norm_rope_bwd(h.a, cus, cur_stream());
+  return {dq, dk, dqw, dkw};
 }
 
 at::Tensor as_int(const at::Tensor& t) { return t.to(at::kInt).contiguous(); }
@@ -294,6 +411,8 @@ void bind_contrib(pybind11::module_& root) {
   pm.def("max_group", &peer_max_group);
   pm.def("allgather", &pm_allgather);
   auto t = root.def_submodule("fused_transformer", "transformer block elementwise fusions (gfx950)");
+  t.def("qk_norm_rope_forward", &qk_forward);
+  t.def("qk_norm_rope_backward", &qk_backward);
   t.def("bias_dropout_add_forward", &bda_forward, pybind11::arg("x"), pybind11::arg("bias"), pybind11::arg("residual"),
         pybind11::arg("p"), pybind11::arg("seed"), pybind11::arg("offset"), pybind11::arg("rng_step") = c10::nullopt);
   t.def("bias_dropout_add_backward", &bda_backward, pybind11::arg("grad"), pybind11::arg("p"), pybind11::arg("seed"),
