@@ -3,6 +3,7 @@
 // max_log_sum_exp]; backward(grad_loss, logits, max_log_sum_exp, labels, smoothing)).
 // The padding-index masking the reference does in python is folded into the kernels here.
 #include "common.h"
+#include "apex_amd/topk_distill_api.h"
 
 namespace apex_amd {
 
@@ -44,6 +45,74 @@ at::Tensor bwd(const at::Tensor& grad_loss, const at::Tensor& logits, const at::
   return grad;
 }
 
+// ---- distillation from a teacher's top logits (csrc/xentropy/topk_distill.hip) ----
+struct DistillHold {
+  TopkDistillArgs a{};
+  at::Tensor x, tz, ti;
+};
+
+void distill_setup(DistillHold& h, const at::Tensor& logits, const at::Tensor& tz, const at::Tensor& ti, double temperature) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) > 0,
+              "topk_distill: [rows, classes] GPU logits expected");
+  TORCH_CHECK(tz.is_cuda() && ti.is_cuda() && tz.get_device() == logits.get_device() &&
+                  ti.get_device() == logits.get_device() && tz.dim() == 2 && tz.sizes() == ti.sizes() &&
+                  tz.size(0) == logits.size(0) && tz.size(1) <= kDistillMaxTop,
+              "topk_distill: teacher logits and indices must be [rows, top <= ", kDistillMaxTop, "] on the logits' device");
+  TORCH_CHECK(ti.scalar_type() == at::kLong || ti.scalar_type() == at::kInt,
+              "topk_distill: teacher indices must be int64 or int32");
+  TORCH_CHECK(logits.size(1) < (int64_t(1) << 30) && logits.size(0) <= kDistillMaxRows,
+              "topk_distill: too many rows or classes");
+  TORCH_CHECK(temperature > 0, "topk_distill: the temperature must be positive");
+  // rows of any pitch are read in place; other layouts are copied
+  h.x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
+  h.tz = tz.contiguous().to(at::kFloat);
+  h.ti = ti.contiguous();
+  TopkDistillArgs& a = h.a;
+  a.logits = h.x.data_ptr();
+  a.pitch = h.x.stride(0);
+  a.rows = h.x.size(0);
+  a.classes = (int)h.x.size(1);
+  a.top = (int)tz.size(1);
+  a.teacher_logits = h.tz.data_ptr<float>();
+  a.teacher_indices = h.ti.data_ptr();
+  a.index64 = h.ti.scalar_type() == at::kLong;
+  a.temperature = (float)temperature;
+  a.dtype = dtype_code(h.x.scalar_type());
+}
+
+std::vector<at::Tensor> distill_fwd(const at::Tensor& logits, const at::Tensor& tz, const at::Tensor& ti,
+                                    double temperature) {
+  TORCH_CHECK(logits.is_cuda(), "topk_distill: GPU logits expected");
+  const c10::hip::HIPGuard g(logits.get_device());
+  DistillHold h;
+  distill_setup(h, logits, tz, ti, temperature);
+  auto fo = logits.options().dtype(at::kFloat);
+  auto losses = at::empty({h.a.rows}, fo), stats = at::empty({h.a.rows, 2}, fo);
+  const int cus = device_cus(logits.get_device());
+  auto parts = at::empty({topk_distill_part_floats(h.a, cus)}, fo);
+  topk_distill_fwd(h.a, losses.data_ptr<float>(), stats.data_ptr<float>(), parts.data_ptr<float>(), cus, cur_stream());
+  return {losses, stats};
+}
+
+at::Tensor distill_bwd(const at::Tensor& grad_loss, const at::Tensor& logits, const at::Tensor& stats,
+                       const at::Tensor& tz, const at::Tensor& ti, double temperature) {
+  TORCH_CHECK(logits.is_cuda(), "topk_distill: GPU logits expected");
+  const c10::hip::HIPGuard g(logits.get_device());
+  DistillHold h;
+  distill_setup(h, logits, tz, ti, temperature);
+  auto on_rows = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.get_device() == logits.get_device() && t.dim() >= 1 && t.size(0) == h.a.rows;
+  };
+  TORCH_CHECK(on_rows(grad_loss) && grad_loss.dim() == 1 && on_rows(stats) && stats.numel() == 2 * h.a.rows &&
+                  stats.scalar_type() == at::kFloat && stats.is_contiguous(),
+              "topk_distill: [rows] grad_loss and [rows, 2] statistics on the logits' device expected");
+  at::Tensor gl = grad_loss.to(at::kFloat);  // any stride (a broadcast gradient has stride 0)
+  auto grad = at::empty(logits.sizes(), logits.options());
+  topk_distill_bwd(h.a, gl.data_ptr<float>(), gl.stride(0), stats.data_ptr<float>(), grad.data_ptr(),
+                   device_cus(logits.get_device()), cur_stream());
+  return grad;
+}
+
 }  // namespace
 
 void bind_xentropy(pybind11::module_& root) {
@@ -53,6 +122,10 @@ void bind_xentropy(pybind11::module_& root) {
         py::arg("padding_idx") = c10::nullopt);
   m.def("backward", &bwd, py::arg("grad_loss"), py::arg("logits"), py::arg("max_log_sum_exp"), py::arg("labels"),
         py::arg("smoothing"), py::arg("padding_idx") = c10::nullopt);
+  m.def("topk_distill_forward", &distill_fwd, py::arg("logits"), py::arg("teacher_logits"), py::arg("teacher_indices"),
+        py::arg("temperature"));
+  m.def("topk_distill_backward", &distill_bwd, py::arg("grad_loss"), py::arg("logits"), py::arg("stats"),
+        py::arg("teacher_logits"), py::arg("teacher_indices"), py::arg("temperature"));
 }
 
 }  // namespace apex_amd

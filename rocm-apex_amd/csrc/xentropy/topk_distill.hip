@@ -1,0 +1,316 @@
+// Distillation loss against a teacher's top logits (forward + backward) for gfx950.
+//
+// Teacher: `top` logits z_k at classes j_k of a row (j_k < 0: no entry), t = softmax over the
+// valid entries of z / T.  Student: q = softmax(x / T) over all classes.
+//   loss = T^2 sum_k t_k (log t_k - log q_{j_k})          (T^2 KL(t || q); 0 for a row without entries)
+//   dx_v = g T (q_v - sum_k t_k [j_k = v])
+//
+// Both passes are bound by the logits' bytes: the forward reads them once (running maximum and
+// rescaled sum per lane over 8-element vectors, in base 2 with 1/T folded into its scale), the
+// backward reads them once and writes the gradient once.  Rows of any pitch and alignment (odd
+// vocabularies) take the same 16-byte accesses at element-aligned addresses.
+// A row is one workgroup when there are rows enough to fill the chip; fewer rows are split over
+// workgroups, (maximum, sum) pairs of the parts joined in a fixed order by a second launch.
+// In the backward the workgroup that wrote a class's dense value also writes the teacher's
+// correction to it (after a barrier), so no atomics: entries naming one class twice are summed by
+// the first of them.
+// A class index past the vocabulary makes the row's loss and gradient NaN; nothing is read there.
+// Row statistics, teacher weights and losses are fp32.  The backward gets the row's (maximum, sum)
+// pair rather than their log-sum-exp: 2^((x - maximum) c) / sum keeps the digits that rounding
+// maximum + log(sum) to 24 bits loses (about 1e-6 of q at logits of 30).
+#include <climits>
+
+#include "apex_amd/device.h"
+#include "apex_amd/dispatch.h"
+#include "apex_amd/topk_distill_api.h"
+
+namespace apex_amd {
+namespace kd {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Pack8 { T e[8]; };
+
+template <typename T>
+__device__ __forceinline__ void load8(float (&r)[8], const T* p) {
+  const Pack8<T> v = *reinterpret_cast<const Pack8<T>*>(p);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = to_f(v.e[i]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&r)[8]) {
+  Pack8<T> v;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v.e[i] = from_f<T>(r[i]);
+  *reinterpret_cast<Pack8<T>*>(p) = v;
+}
+
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// (m, s): m the maximum so far, s = sum 2^((x - m) c), c = log2(e) / T.  The subtraction comes before
+// the scale, so the error of an exponent is relative to x - m (exact at the maximum), not to x.  A maximum
+// of -inf (nothing or only -inf so far) subtracts 0 instead, so -inf - -inf never appears; NaN reaches s.
+__device__ __forceinline__ float base(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ void merge(float& m, float& s, float m2, float s2, float c) {
+  const float M = fmaxf(m, m2), b = base(M);
+  s = s * exp2_((m - b) * c) + s2 * exp2_((m2 - b) * c);
+  m = M;
+}
+
+template <int N>
+__device__ __forceinline__ void accumulate(float& m, float& s, const float (&x)[N], float c) {
+  float lm = x[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) lm = fmaxf(lm, x[k]);
+  const float M = fmaxf(m, lm), b = base(M);
+  float ls = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) ls += exp2_((x[k] - b) * c);
+  s = s * exp2_((m - b) * c) + ls;
+  m = M;
+}
+
+// Teacher weights of a row into LDS: cls[k] (-1: none) and t[k]; also log2 t in lt (forward).
+// Returns the row's state in every thread: 0 no entries, 1 usable, 2 a class past the vocabulary.
+// All threads call it; `red` holds 2 * kWaves floats.
+template <typename TI>
+__device__ __forceinline__ int teacher_row(const float* __restrict__ z, const TI* __restrict__ idx, int top, int classes,
+                                           float c, int* cls, float* t, float* lt, float* red) {
+  float m = -INFINITY;
+  int state = 0;
+  for (int k = threadIdx.x; k < top; k += kThreads) {
+    const int64_t j = (int64_t)idx[k];
+    const bool in = j >= 0 && j < classes;
+    if (j >= 0) state |= in ? 1 : 2;
+    const float y = in ? z[k] : -INFINITY;
+    cls[k] = in ? (int)j : -1;
+    t[k] = y;
+    m = fmaxf(m, y);
+  }
+  m = block_max(m, red);
+  const float b = base(m);
+  float s = 0.f;
+  for (int k = threadIdx.x; k < top; k += kThreads) s += exp2_((t[k] - b) * c);
+  s = block_sum(s, red);
+  const float inv = 1.f / s, ls = __builtin_amdgcn_logf(s);
+  for (int k = threadIdx.x; k < top; k += kThreads) {
+    const float y = (t[k] - b) * c;
+    if (lt != nullptr) lt[k] = y - ls;
+    t[k] = s == 0.f ? 0.f : exp2_(y) * inv;
+  }
+  const int any = __syncthreads_or(state & 1), bad = __syncthreads_or(state & 2);
+  return bad ? 2 : (any && s != 0.f) ? 1 : 0;
+}
+
+// the row's loss and its (maximum, sum), from the latter (thread 0 writes)
+template <typename T>
+__device__ __forceinline__ void row_loss(const T* __restrict__ x, float m, float s, float c, float temp, int state,
+                                         int top, const int* cls, const float* t, const float* lt, float* red,
+                                         float* __restrict__ loss, float2* __restrict__ stat) {
+  const float ls = __builtin_amdgcn_logf(s);
+  float a = 0.f;
+  if (state == 1)
+    for (int k = threadIdx.x; k < top; k += kThreads)
+      if (cls[k] >= 0 && t[k] != 0.f) a += t[k] * (lt[k] - ((to_f(x[cls[k]]) - m) * c - ls));
+  a = block_sum(a, red);
+  if (threadIdx.x == 0) {
+    *loss = state == 2 ? __builtin_nanf("") : temp * temp * 0.6931471805599453f * a;
+    *stat = make_float2(m, s);
+  }
+}
+
+// One (row, part): the part's (maximum, sum); a row in one part also gets its loss here.
+template <typename T, typename TI>
+__global__ void __launch_bounds__(kThreads)
+kd_fwd_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const float* __restrict__ tz,
+              const TI* __restrict__ ti, int top, float c, float temp, float* __restrict__ losses,
+              float2* __restrict__ stats, float2* __restrict__ parts, int chunk) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ float red[2 * kWaves];
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * pitch;
+  const int c0 = blockIdx.y * chunk, c1 = min(classes, c0 + chunk);
+  float m = -INFINITY, s = 0.f;
+  int v = c0 + threadIdx.x * 8;
+  for (; v + 8 * kThreads + 8 <= c1; v += 16 * kThreads) {  // two vectors in flight
+    float r0[8], r1[8];
+    load8<T>(r0, x + v);
+    load8<T>(r1, x + v + 8 * kThreads);
+    accumulate<8>(m, s, r0, c);
+    accumulate<8>(m, s, r1, c);
+  }
+  for (; v + 8 <= c1; v += 8 * kThreads) {
+    float r0[8];
+    load8<T>(r0, x + v);
+    accumulate<8>(m, s, r0, c);
+  }
+  for (int e = c0 + ((c1 - c0) & ~7) + threadIdx.x; e < c1; e += kThreads) {
+    const float r1[1] = {to_f(x[e])};
+    accumulate<1>(m, s, r1, c);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) merge(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6] = m;
+    red[kWaves + (threadIdx.x >> 6)] = s;
+  }
+  __syncthreads();
+  m = red[0];
+  s = red[kWaves];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) merge(m, s, red[w], red[kWaves + w], c);
+  __syncthreads();
+  if (parts != nullptr) {
+    if (threadIdx.x == 0) parts[row * gridDim.y + blockIdx.y] = make_float2(m, s);
+    return;
+  }
+  int* cls = (int*)lds;
+  float *t = lds + top, *lt = lds + 2 * top;
+  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, lt, red);
+  row_loss(x, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
+}
+
+// join a row's parts (fixed order) and take its loss
+template <typename T, typename TI>
+__global__ void __launch_bounds__(kThreads)
+kd_join_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const float* __restrict__ tz,
+               const TI* __restrict__ ti, int top, float c, float temp, float* __restrict__ losses,
+               float2* __restrict__ stats, const float2* __restrict__ parts, int nparts) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ float red[2 * kWaves];
+  const int64_t row = blockIdx.x;
+  float m = -INFINITY, s = 0.f;
+  for (int i = threadIdx.x & 63; i < nparts; i += 64) {
+    const float2 p = parts[row * nparts + i];
+    merge(m, s, p.x, p.y, c);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) merge(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
+  int* cls = (int*)lds;
+  float *t = lds + top, *lt = lds + 2 * top;
+  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, lt, red);
+  row_loss(logits + row * pitch, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
+}
+
+template <typename T, typename TI>
+__global__ void __launch_bounds__(kThreads)
+kd_bwd_kernel(const float* __restrict__ gl, int64_t gl_stride, const T* __restrict__ logits, int64_t pitch, int classes,
+              const float* __restrict__ tz, const TI* __restrict__ ti, int top, float c, float temp,
+              const float2* __restrict__ stats, T* __restrict__ grad, int chunk) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ float red[2 * kWaves];
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * pitch;
+  T* gx = grad + row * classes;
+  const int c0 = blockIdx.y * chunk, c1 = min(classes, c0 + chunk);
+  int* cls = (int*)lds;
+  float* t = lds + top;
+  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, nullptr, red);
+  const float2 st = stats[row];
+  const float b = base(st.x);
+  const float coef = state == 2 ? __builtin_nanf("") : gl[row * gl_stride] * temp;
+  const float pc = coef / st.y;  // q_v = 2^((x - max) c) / sum
+  const int tail = c0 + ((c1 - c0) & ~7);
+  if (state == 0) {  // no teacher: a zero row whatever the logits and the incoming gradient hold
+    const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int v = c0 + threadIdx.x * 8; v + 8 <= c1; v += 8 * kThreads) store8<T>(gx + v, zero);
+    for (int e = tail + threadIdx.x; e < c1; e += kThreads) gx[e] = from_f<T>(0.f);
+    return;
+  }
+  for (int v = c0 + threadIdx.x * 8; v + 8 <= c1; v += 8 * kThreads) {
+    float r[8];
+    load8<T>(r, x + v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r[k] = pc * exp2_((r[k] - b) * c);
+    store8<T>(gx + v, r);
+  }
+  for (int e = tail + threadIdx.x; e < c1; e += kThreads) gx[e] = from_f<T>(pc * exp2_((to_f(x[e]) - b) * c));
+  __syncthreads();
+  for (int k = threadIdx.x; k < top; k += kThreads) {
+    const int j = cls[k];
+    if (j < c0 || j >= c1) continue;
+    float sum = 0.f;
+    bool first = true;
+    for (int i = 0; i < top; ++i)
+      if (cls[i] == j) {
+        first = first && i >= k;
+        sum += t[i];
+      }
+    if (first) gx[j] = from_f<T>(pc * exp2_((to_f(x[j]) - b) * c) - coef * sum);
+  }
+}
+
+// parts of a row: one when the rows alone give every CU 4 workgroups, else enough for that, at
+// least 4096 classes each (16 vectors a lane... a shorter part is mostly launch and reduction)
+inline int row_parts(int64_t rows, int classes, int cus, int* chunk) {
+  int64_t p = rows >= (int64_t)cus * 4 ? 1 : ((int64_t)cus * 4 + rows - 1) / rows;
+  const int64_t most = classes / 4096 > 1 ? classes / 4096 : 1;
+  if (p > most) p = most;
+  const int64_t each = ((int64_t)classes + p - 1) / p;
+  *chunk = (int)((each + 2047) / 2048 * 2048);
+  return (int)(((int64_t)classes + *chunk - 1) / *chunk);
+}
+
+template <typename F>
+void dispatch(const TopkDistillArgs& a, F&& f) {
+  dispatch_float(a.dtype, [&](auto tag) {
+    if (a.index64) f(tag, Tag<int64_t>{});
+    else f(tag, Tag<int32_t>{});
+  }, "topk_distill");
+}
+
+inline void check(const TopkDistillArgs& a) {
+  if (a.rows < 0 || a.rows > kDistillMaxRows || a.classes < 1 || a.classes > INT_MAX - (1 << 16) || a.top < 0 || a.top > kDistillMaxTop)
+    throw std::runtime_error("topk_distill: sizes out of range");
+}
+
+}  // namespace kd
+
+int64_t topk_distill_part_floats(const TopkDistillArgs& a, int cus) {
+  int chunk;
+  const int p = a.rows > 0 ? kd::row_parts(a.rows, a.classes, cus, &chunk) : 1;
+  return p > 1 ? 2 * a.rows * p : 0;
+}
+
+void topk_distill_fwd(const TopkDistillArgs& a, float* losses, float* stats, float* parts, int cus, hipStream_t s) {
+  kd::check(a);
+  if (a.rows == 0) return;
+  int chunk;
+  const int p = kd::row_parts(a.rows, a.classes, cus, &chunk);
+  const size_t lds = (size_t)3 * a.top * sizeof(float);
+  const float c = 1.4426950408889634f / a.temperature;
+  kd::dispatch(a, [&](auto tag, auto itag) {
+    using T = typename decltype(tag)::type;
+    using TI = typename decltype(itag)::type;
+    hipLaunchKernelGGL((kd::kd_fwd_kernel<T, TI>), dim3((unsigned)a.rows, p), dim3(kd::kThreads), p > 1 ? 0 : lds, s,
+                       (const T*)a.logits, a.pitch, a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top, c,
+                       a.temperature, losses, (float2*)stats, p > 1 ? (float2*)parts : (float2*)nullptr, chunk);
+    if (p > 1)
+      hipLaunchKernelGGL((kd::kd_join_kernel<T, TI>), dim3((unsigned)a.rows), dim3(kd::kThreads), lds, s,
+                         (const T*)a.logits, a.pitch, a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top,
+                         c, a.temperature, losses, (float2*)stats, (const float2*)parts, p);
+  });
+  check_launch("topk_distill forward");
+}
+
+void topk_distill_bwd(const TopkDistillArgs& a, const float* grad_loss, int64_t grad_loss_stride, const float* stats,
+                      void* grad, int cus, hipStream_t s) {
+  kd::check(a);
+  if (a.rows == 0) return;
+  int chunk;
+  const int p = kd::row_parts(a.rows, a.classes, cus, &chunk);
+  const float c = 1.4426950408889634f / a.temperature;
+  kd::dispatch(a, [&](auto tag, auto itag) {
+    using T = typename decltype(tag)::type;
+    using TI = typename decltype(itag)::type;
+    hipLaunchKernelGGL((kd::kd_bwd_kernel<T, TI>), dim3((unsigned)a.rows, p), dim3(kd::kThreads),
+                       (size_t)2 * a.top * sizeof(float), s, grad_loss, grad_loss_stride, (const T*)a.logits, a.pitch,
+                       a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top, c, a.temperature,
+                       (const float2*)stats, (T*)grad, chunk);
+  });
+  check_launch("topk_distill backward");
+}
+
+}  // namespace apex_amd
