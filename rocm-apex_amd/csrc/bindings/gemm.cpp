@@ -6,6 +6,7 @@
 // Every GEMM of a Linear layer (forward, input gradient, weight gradient) is one launch of the
 // same kernel family; no operand is transposed in memory.
 #include "common.h"
+#include "apex_amd/gated_ffn_api.h"
 #include "apex_amd/gemm_api.h"
 
 namespace apex_amd {
@@ -116,6 +117,126 @@ at::Tensor linear_wgrad(const at::Tensor& dy2, const at::Tensor& x2) {
                   nullptr);
 }
 
+// ---- gated feed-forward block (csrc/gemm/gated_ffn.hip) ----
+// contiguous, and 16-byte aligned even where a contiguous view starts inside a vector
+at::Tensor vec16(const at::Tensor& t) {
+  at::Tensor c = t.contiguous();
+  return ((uintptr_t)c.data_ptr() & 15u) ? c.clone() : c;
+}
+
+void ffn_run(int op, const at::Tensor& a, bool a_kmajor, const at::Tensor& b, bool b_kmajor, int64_t m, int64_t n,
+             int64_t k, const at::Tensor& c, int act, const at::Tensor& bias, const at::Tensor& aux_in,
+             const at::Tensor& aux_out) {
+  TORCH_CHECK(m < (int64_t(1) << 31) && n < (int64_t(1) << 30) && k < (int64_t(1) << 31), "gated_ffn: sizes too large");
+  FfnArgs g{};
+  g.a = a.data_ptr();
+  g.b = b.data_ptr();
+  g.c = c.data_ptr();
+  g.m = (int)m;
+  g.n = (int)n;
+  g.k = (int)k;
+  g.a_kmajor = a_kmajor;
+  g.b_kmajor = b_kmajor;
+  g.lda = a.size(1);
+  g.ldb = b.size(1);
+  g.ldc = c.size(1);
+  g.dtype = dtype_code(a.scalar_type());
+  g.op = op;
+  g.act = act;
+  g.bias = bias.defined() ? bias.data_ptr() : nullptr;
+  g.aux_in = aux_in.defined() ? aux_in.data_ptr() : nullptr;
+  g.aux_out = aux_out.defined() ? aux_out.data_ptr() : nullptr;
+  TORCH_CHECK(ffn_supported(g), "gated_ffn: unsupported sizes or alignment (fp16 / bf16, widths multiples of 8)");
+  const int cus = device_cus(a.get_device());
+  at::Tensor ws;
+  const int64_t wsf = ffn_workspace_floats(g, cus);
+  if (wsf > 0) {
+    ws = at::empty({wsf}, a.options().dtype(at::kFloat));
+    g.ws = ws.data_ptr<float>();
+  }
+  ffn_gemm(g, cus, cur_stream());
+}
+
+void ffn_check(const at::Tensor& x, const at::Tensor& w1, const at::Tensor& w2, int64_t act) {
+  auto ok = [&](const at::Tensor& t) {
+    return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == x.scalar_type() && t.dim() == 2;
+  };
+  TORCH_CHECK(ok(x) && ok(w1) && ok(w2) && w1.size(1) == x.size(1) && w1.size(0) == 2 * w2.size(1),
+              "gated_ffn: [m, k] input, [2f, k] weight1 and [n, f] weight2 of one dtype and device expected");
+  TORCH_CHECK(act == kGateSilu || act == kGateGelu, "gated_ffn: unknown activation");
+}
+
+at::Tensor ffn_bias(const OT& b, int64_t n, const at::Tensor& x) {
+  if (!has(b)) return at::Tensor();
+  TORCH_CHECK(b->is_cuda() && b->get_device() == x.get_device() && b->scalar_type() == x.scalar_type() &&
+                  b->numel() == n,
+              "gated_ffn: bias size, dtype or device mismatch");
+  return vec16(*b);
+}
+
+// (y, h, au); h and au (the backward's inputs) are undefined unless save
+std::vector<at::Tensor> ffn_forward(const at::Tensor& x_, const at::Tensor& w1_, const OT& b1_, const at::Tensor& w2_,
+                                    const OT& b2_, int64_t act, bool save) {
+  TORCH_CHECK(x_.is_cuda(), "gated_ffn: GPU tensors expected");
+  const c10::hip::HIPGuard guard(x_.get_device());
+  ffn_check(x_, w1_, w2_, act);
+  at::Tensor x = vec16(x_), w1 = vec16(w1_), w2 = vec16(w2_);
+  const int64_t m = x.size(0), k = x.size(1), f = w2.size(1), n = w2.size(0);
+  at::Tensor b1 = ffn_bias(b1_, 2 * f, x), b2 = ffn_bias(b2_, n, x);
+  at::Tensor h = at::empty({m, f}, x.options()), y = at::empty({m, n}, x.options()), au;
+  if (save) au = at::empty({m, 2 * f}, x.options());
+  if (m > 0) {
+    ffn_run(kFfnGated, x, true, w1, true, m, f, k, h, (int)act, b1, at::Tensor(), au);
+    ffn_run(kFfnPlain, h, true, w2, true, m, n, f, y, 0, b2, at::Tensor(), at::Tensor());
+  }
+  return {y, save ? h : at::Tensor(), au};
+}
+
+// (dx, dw1, db1, dw2, db2), undefined where not needed
+std::vector<at::Tensor> ffn_backward(const at::Tensor& dy_, const at::Tensor& x_, const at::Tensor& w1_,
+                                     const at::Tensor& w2_, const at::Tensor& h, const at::Tensor& au, int64_t act,
+                                     bool need_dx, bool need_dw1, bool need_db1, bool need_dw2, bool need_db2) {
+  TORCH_CHECK(x_.is_cuda(), "gated_ffn: GPU tensors expected");
+  const c10::hip::HIPGuard guard(x_.get_device());
+  ffn_check(x_, w1_, w2_, act);
+  at::Tensor dy = vec16(dy_), x = vec16(x_), w1 = vec16(w1_), w2 = vec16(w2_);
+  const int64_t m = x.size(0), k = x.size(1), f = w2.size(1), n = w2.size(0);
+  auto is = [&](const at::Tensor& t, int64_t c) {
+    return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == x.scalar_type() && t.dim() == 2 &&
+           t.size(0) == m && t.size(1) == c && t.is_contiguous();
+  };
+  TORCH_CHECK(is(dy, n) && is(h, f) && is(au, 2 * f), "gated_ffn: backward operands do not fit");
+  const at::Tensor none;
+  at::Tensor dx, dw1, db1, dw2, db2;
+  if (m == 0) {
+    if (need_dx) dx = at::empty({0, k}, x.options());
+    if (need_dw1) dw1 = at::zeros_like(w1);
+    if (need_db1) db1 = at::zeros({2 * f}, x.options());
+    if (need_dw2) dw2 = at::zeros_like(w2);
+    if (need_db2) db2 = at::zeros({n}, x.options());
+    return {dx, dw1, db1, dw2, db2};
+  }
+  if (need_dw2) {
+    dw2 = at::empty({n, f}, x.options());
+    ffn_run(kFfnPlain, dy, false, h, false, n, f, m, dw2, 0, none, none, none);
+  }
+  if (need_db2) db2 = colsum(dy, x.scalar_type());
+  if (need_dx || need_dw1 || need_db1) {
+    at::Tensor dau = at::empty({m, 2 * f}, x.options());
+    ffn_run(kFfnDGated, dy, true, w2, false, m, f, n, dau, (int)act, none, au, none);
+    if (need_dw1) {
+      dw1 = at::empty({2 * f, k}, x.options());
+      ffn_run(kFfnPlain, dau, false, x, false, 2 * f, k, m, dw1, 0, none, none, none);
+    }
+    if (need_db1) db1 = colsum(dau, x.scalar_type());
+    if (need_dx) {
+      dx = at::empty({m, k}, x.options());
+      ffn_run(kFfnPlain, dau, true, w1, false, m, k, 2 * f, dx, 0, none, none, none);
+    }
+  }
+  return {dx, dw1, db1, dw2, db2};
+}
+
 }  // namespace
 
 void bind_lt(pybind11::module_& root);  // lt_epilogue.cpp
@@ -194,6 +315,12 @@ void bind_gemm(pybind11::module_& root) {
   g.def("column_sum", [](at::Tensor x, c10::optional<at::ScalarType> out_dtype) {
     return colsum(as2d(x), out_dtype.value_or(x.scalar_type()));
   }, py::arg("x"), py::arg("out_dtype") = c10::nullopt);
+
+  auto gf = root.def_submodule("gated_ffn", "gated feed-forward block on gfx950 MFMA");
+  gf.attr("ACT_SILU") = (int)kGateSilu;
+  gf.attr("ACT_GELU") = (int)kGateGelu;
+  gf.def("forward", &ffn_forward);
+  gf.def("backward", &ffn_backward);
 
   auto fd = root.def_submodule("fused_dense_cuda", "fused dense (GEMM + bias [+ GeLU]) on gfx950 MFMA");
   fd.def("linear_bias_forward", [](at::Tensor input, at::Tensor weight, OT bias) {

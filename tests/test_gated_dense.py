@@ -1,0 +1,244 @@
+"""Gated feed-forward block against its formulas in 64 bits.
+
+Tolerances.  Let e = eps/2 of the type (one rounding) and G = 2^-23 * sqrt-free bound of an fp32 sum: a
+k-term product sum in MFMA steps errs by at most (k/16 + 16) 2^-24 of the sum of its terms' magnitudes.
+h, au, da and du are rounded to the type between the products, so each output's error is bounded by the
+64-bit sum of its terms' magnitudes, times the roundings its terms carry:
+  y: h (1)                                 dW2: h (1)
+  da, du (so dx, dW1, db1): a and u rounded, the gradient rounded: u (1), act'(a) or act(a), whose
+  change over a rounding of a is at most e |a| sup|act''| (0.5 for silu, 1.13 for gelu) or e |a| sup|act'|
+  (1.1), and its own rounding (1).  Measured against magnitudes |dh| |u| (|act'| + 1.13 |a|) and
+  |dh| (|act| + 1.1 |a|) this is at most 3 e.
+and one rounding (e) of the output itself."""
+import math
+
+import pytest
+import torch
+
+from apex.fused_dense import FusedDenseGatedDense, fused_dense_gated_dense_function
+
+
+def _act(a, kind):
+    if kind == "silu":
+        s = torch.sigmoid(a)
+        return a * s, s * (1 + a * (1 - s))
+    c0, c1 = math.sqrt(2 / math.pi), 0.044715
+    th = torch.tanh(c0 * (a + c1 * a ** 3))
+    return 0.5 * a * (1 + th), 0.5 * (1 + th) + 0.5 * a * (1 - th * th) * c0 * (1 + 3 * c1 * a * a)
+
+
+def _exact(x, w1, b1, w2, b2, kind, dy):
+    """[(value, magnitude of its terms, roundings, summed length)] of y, dx, dw1, db1, dw2, db2."""
+    x, w1, w2, dy = (t.detach().double().cpu() for t in (x, w1, w2, dy))
+    f = w2.size(1)
+    au = x @ w1.t() + (0 if b1 is None else b1.detach().double().cpu())
+    a, u = au[:, :f], au[:, f:]
+    act, dact = _act(a, kind)
+    h = act * u
+    # an fp32 sum of k terms behind a and u enters everything after them; it is far below e of the type
+    y = h @ w2.t() + (0 if b2 is None else b2.detach().double().cpu())
+    dh = dy @ w2
+    dau = torch.cat((dh * u * dact, dh * act), 1)
+    dhm = dy.abs() @ w2.abs()
+    # dh's own fp32 error is relative to dhm; the roundings of a, u, da, du to |dh| (dhm >= |dh|)
+    mag = torch.cat((dh.abs() * u.abs() * (dact.abs() + 1.13 * a.abs()), dh.abs() * (act.abs() + 1.1 * a.abs())), 1)
+    sums = torch.cat((dhm * u.abs() * dact.abs(), dhm * act.abs()), 1)
+    hm = h.abs() + (1.1 * a.abs() * u.abs())
+    m, k = x.shape
+    n = w2.size(0)
+    return {
+        "y": (y, hm @ w2.abs().t(), 1, f, 0),
+        "dx": (dau @ w1, mag @ w1.abs(), 3, 2 * f, sums @ w1.abs()),
+        "dw1": (dau.t() @ x, mag.t() @ x.abs(), 3, m, sums.t() @ x.abs()),
+        "db1": (dau.sum(0), mag.sum(0), 3, m, sums.sum(0)),
+        "dw2": (dy.t() @ h, dy.abs().t() @ hm, 1, m, 0),
+        "db2": (dy.sum(0), dy.abs().sum(0), 0, m, 0),
+    }
+
+
+def _close(got, want, mag, roundings, length, sums, k, what):
+    e = torch.finfo(got.dtype).eps / 2
+    f32 = 2.0 ** -24
+    bound = 1.01 * e * want.abs() + mag * (roundings * e + (length / 16 + k / 16 + 48) * f32) + sums * (k / 16 + 16) * f32
+    bound = bound + (2.0 ** -24 if got.dtype == torch.float16 else 0.0)
+    ratio = ((got.detach().double().cpu() - want).abs() / bound.clamp(min=1e-300)).max()
+    assert got.isfinite().all() and ratio <= 1, f"{what}: {float(ratio):.3f} bounds"
+
+
+def _inputs(dev, m, k, f, n, dtype, bias, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s, std=1.0: (torch.randn(*s, generator=g) * std).to(dtype).to(dev)
+    x, w1, w2 = rnd(m, k), rnd(2 * f, k, std=k ** -0.5), rnd(n, f, std=f ** -0.5)
+    b1, b2 = (rnd(2 * f, std=0.3), rnd(n, std=0.3)) if bias else (None, None)
+    for t in (x, w1, w2, b1, b2):
+        if t is not None:
+            t.requires_grad_(True)
+    return x, w1, b1, w2, b2, rnd(m, n)
+
+
+def _check(x, w1, b1, w2, b2, dy, kind):
+    y = fused_dense_gated_dense_function(x, w1, b1, w2, b2, kind)
+    leaves = dict(dx=x, dw1=w1, db1=b1, dw2=w2, db2=b2)
+    leaves = {a: t for a, t in leaves.items() if t is not None}
+    grads = torch.autograd.grad(y, list(leaves.values()), dy)
+    want = _exact(x, w1, b1, w2, b2, kind, dy)
+    k = max(x.size(1), w2.size(0))
+    _close(y, *want["y"], k, "y")
+    for name, g in zip(leaves, grads):
+        _close(g, *want[name], k, name)
+    with torch.no_grad():
+        assert torch.equal(fused_dense_gated_dense_function(x, w1, b1, w2, b2, kind), y)
+
+
+def test_cpu_block_and_module():
+    for kind in ("silu", "gelu"):
+        _check(*_inputs("cpu", 5, 12, 7, 9, torch.float32, True), kind)
+        m = FusedDenseGatedDense(6, 10, 4, bias=True, activation=kind).double()
+        x = torch.randn(2, 3, 6, dtype=torch.float64, requires_grad=True)
+        assert torch.autograd.gradcheck(lambda x, *p: fused_dense_gated_dense_function(x, p[0], p[2], p[1], p[3], kind),
+                                        (x, m.weight1, m.weight2, m.bias1, m.bias2))
+        assert m(x).shape == (2, 3, 4) and FusedDenseGatedDense(6, 10, 4).bias1 is None
+
+
+def _refusals(dev):
+    f = fused_dense_gated_dense_function
+    z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device=dev)
+    x, w1, w2 = z(3, 8), z(32, 8), z(8, 16)
+    f(x, w1, None, w2, None)
+    for err, args in [(ValueError, (x, w1, None, w2, None, "relu")), (ValueError, (x, z(31, 8), None, w2, None)),
+                      (ValueError, (z(3, 9), w1, None, w2, None)), (ValueError, (x, w1, z(16), w2, None)),
+                      (ValueError, (x, w1, None, w2, z(9))), (TypeError, (x, w1.half(), None, w2, None)),
+                      (TypeError, (x, w1, z(32, dt=torch.bfloat16), w2, None)), (ValueError, (x, w1[0], None, w2, None)),
+                      (ValueError, (x, z(0, 8), None, z(8, 0), None))]:
+        with pytest.raises(err):
+            f(*args)
+    with pytest.raises(ValueError):
+        FusedDenseGatedDense(4, 4, 4, activation="tanh")
+
+
+def test_cpu_refusals():
+    _refusals("cpu")
+
+
+# ------------------------------------------------------------------------------------------- GPU
+# one token; odd row counts around the tiles; widths that end inside a 16-byte k step, a 64-deep tile,
+# a tile; splits over the tokens; several tiles each way
+SHAPES = [(1, 8, 8, 8), (1, 256, 136, 64), (3, 64, 128, 72), (17, 72, 264, 136), (33, 512, 1000, 256), (64, 128, 64, 40),
+          (65, 320, 520, 328), (127, 200, 344, 96), (257, 264, 712, 520), (700, 256, 384, 128), (2100, 136, 200, 72),
+          (4097, 64, 72, 264)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,f,n", SHAPES)
+@pytest.mark.parametrize("kind,bias", [("silu", False), ("gelu", True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gpu_block(m, k, f, n, kind, bias, dtype):
+    _check(*_inputs("cuda", m, k, f, n, dtype, bias), kind)
+
+
+@pytest.mark.gpu
+def test_gpu_layouts_and_leading_axes():
+    x, w1, b1, w2, b2, dy = _inputs("cuda", 60, 64, 96, 48, torch.bfloat16, True)
+    want = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
+    x3 = x.detach().view(3, 4, 5, 64)
+    assert torch.equal(fused_dense_gated_dense_function(x3, w1, b1, w2, b2).view(60, 48), want)
+    # transposed storage, rows of a wider buffer, a view that starts inside a 16-byte vector
+    xt = x.detach().t().contiguous().t()
+    wide = torch.randn(192, 72, device="cuda").to(torch.bfloat16)
+    wide[:, 3:67] = w1.detach()
+    flat = torch.zeros(48 * 96 + 1, device="cuda", dtype=torch.bfloat16)
+    flat[1:] = w2.detach().reshape(-1)
+    wv = flat[1:].view(48, 96)
+    assert torch.equal(fused_dense_gated_dense_function(xt, wide[:, 3:67], b1, wv, b2), want)
+    y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
+    a = torch.autograd.grad(y, [x, w1, w2], dy, retain_graph=True)
+    b = torch.autograd.grad(y, [x, w1, w2], dy.t().contiguous().t(), retain_graph=True)
+    assert all(torch.equal(i, j) for i, j in zip(a, b))
+    c = torch.autograd.grad(y.sum(), [w1])  # an expanded gradient, one leaf only
+    d = torch.autograd.grad(fused_dense_gated_dense_function(x, w1, b1, w2, b2), [w1], torch.ones_like(dy))
+    assert torch.equal(c[0], d[0])
+
+
+@pytest.mark.gpu
+def test_gpu_no_tokens():
+    x, w1, b1, w2, b2, _ = _inputs("cuda", 0, 64, 96, 48, torch.bfloat16, True)
+    y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
+    assert y.shape == (0, 48)
+    y.sum().backward()
+    assert x.grad.shape == (0, 64) and all((t.grad == 0).all() for t in (w1, b1, w2, b2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_gpu_extreme_activations(kind):
+    # gates far out on both sides: act and its derivative saturate, nothing overflows into NaN
+    x = torch.eye(8, device="cuda", dtype=torch.bfloat16)
+    vals = torch.tensor([-1e4, -200.0, -90.0, -20.0, 20.0, 90.0, 200.0, 1e4], device="cuda").to(torch.bfloat16)
+    w1 = torch.cat((vals.expand(8, 8).t(), torch.ones(8, 8, device="cuda", dtype=torch.bfloat16))).contiguous()
+    w2 = torch.eye(8, device="cuda", dtype=torch.bfloat16)
+    w1.requires_grad_(True)
+    y = fused_dense_gated_dense_function(x, w1, None, w2, None, kind)
+    want, dwant = _act(vals.double(), kind)
+    # fp32's exponential overflows past 88.7: a gate below that gives 0 for a value of at most 1e-36
+    torch.testing.assert_close(y.detach().double(), want.expand(8, 8), rtol=1.01 * 2 ** -8, atol=1e-36)
+    dw, = torch.autograd.grad(y, w1, torch.ones_like(y))
+    torch.testing.assert_close(dw[:8].double(), dwant[:, None].expand(8, 8), rtol=2 ** -7, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_gpu_nan_stays_in_its_row():
+    x, w1, b1, w2, b2, dy = _inputs("cuda", 300, 72, 136, 64, torch.bfloat16, False)
+    want = fused_dense_gated_dense_function(x, w1, None, w2, None).detach()
+    with torch.no_grad():
+        x[299] = float("nan")
+        x[7, 3] = float("inf")
+    y = fused_dense_gated_dense_function(x, w1, None, w2, None)
+    keep = torch.ones(300, dtype=torch.bool, device="cuda")
+    keep[[7, 299]] = False
+    assert y[299].isnan().all() and torch.equal(y[keep], want[keep])
+
+
+@pytest.mark.gpu
+def test_gpu_refusals():
+    _refusals("cuda")
+    z = torch.zeros(32, 8, device="cuda")
+    with pytest.raises(ValueError):
+        fused_dense_gated_dense_function(z, z.cpu(), None, torch.zeros(8, 16), None)
+
+
+@pytest.mark.gpu
+def test_gpu_other_types_and_widths_run_the_torch_math():
+    for dtype, shape in ((torch.float32, (9, 24, 40, 16)), (torch.bfloat16, (9, 23, 41, 15))):
+        x, w1, b1, w2, b2, dy = _inputs("cuda", *shape, dtype, True)
+        y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
+        want = _exact(x, w1, b1, w2, b2, "silu", dy)["y"][0]
+        torch.testing.assert_close(y.double().cpu(), want, rtol=0.02, atol=0.05 if dtype != torch.float32 else 1e-4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [20, 1500])
+def test_gpu_other_stream_captured_graph_and_repeatability(m):
+    x, w1, b1, w2, b2, dy = _inputs("cuda", m, 128, 264, 192, torch.bfloat16, True)
+
+    def step():
+        y = fused_dense_gated_dense_function(x, w1, b1, w2, b2, "silu")
+        return [y.detach()] + list(torch.autograd.grad(y, [x, w1, b1, w2, b2], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _check(x, w1, b1, w2, b2, dy, "silu")
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(step(), step()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.mul_(1 - 0.1 * i)
+            w2.add_(0.01 * i)
+        graph.replay()
+        got = [o.clone() for o in outs]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
