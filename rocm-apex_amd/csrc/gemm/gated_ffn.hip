@@ -55,12 +55,26 @@ struct Params {
   int kchunk;
 };
 
-__device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t r, int voff, uint16_t* dst) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)dst, 16, voff, 0, 0, 0);
+// LDS-DMA of 16 bytes a lane to dst + 16 lane.  Written in assembly: behind the builtin the compiler makes
+// every transposing LDS read wait for all DMA in flight (it cannot tell their LDS ranges apart), and the
+// tile that should land during the next four k steps would be waited out in the first.  The waits are
+// the caller's: s_waitcnt vmcnt(0) before the barrier that opens the tile.  No register is written.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void dma(i32x4 r, int voff, uint32_t dst) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know the constraints
+  // m0 is reserved: the compiler sets it right before an instruction that needs it, and this kernel has none
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(voff), "s"(r));
+#endif
 }
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const uint16_t* p, int64_t elems) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)(elems * 2), 0x00027000);
+// raw buffer over `elems` 16-bit elements: loads past them give zeros
+__device__ __forceinline__ i32x4 rsrc(const uint16_t* p, int64_t elems) {
+  const uint64_t b = (uint64_t)p;
+  return i32x4{(int)(uint32_t)b, (int)((uint32_t)(b >> 32) & 0xffffu), (int)(elems * 2), 0x00027000};
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const uint16_t* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint16_t*)p;
 }
 
 // XCD-aware, bijective remap of the linear workgroup id (each XCD gets a contiguous band), then
@@ -77,50 +91,51 @@ __device__ __forceinline__ void tile_coords(int tiles_m, int tiles_n, int& bm, i
   bn = (wgid % (GROUP_M * tiles_n)) / gm;
 }
 
-// One operand's tile of R rows x 64 k into LDS, 1 KB per wave instruction.
+// One operand's tile of R rows x 64 k on its way into LDS, R / 32 instructions of 1 KB a wave.
 // k-major: image [R][64]; 16-byte chunk c of row r at c ^ ((r >> 1) & 7).
 // m-major: image [64][R]; 16-byte chunk c of k row r at c ^ ((r & 3) << 1).
 // Both swizzles spread the rows that one fragment read touches over all banks.
 // GATED (k-major only): image row r is column r % (R/4) of group r / (R/4) = 2 wave + (0 gate, 1 up).
 template <bool KMAJ, int R, bool GATED>
-__device__ __forceinline__ void issue_tile(const uint16_t* __restrict__ X, int64_t ld, int rows, int K, int r0, int k0,
-                                           uint16_t* dst, int wave, int lane) {
-  const int kleft = K - k0;
-  if constexpr (KMAJ) {
-    const int row = 8 * wave + (lane >> 3);               // + 32 i
-    const int c = (lane & 7) ^ ((row >> 1) & 7);
-    const int lane_off = 8 * c < kleft ? (int)((row * ld + 8 * c) * 2) : kOut;
-    if constexpr (!GATED) {
-      const int nr = min(rows - r0, R);
-      const auto rs = rsrc(X + r0 * ld + k0, (nr - 1) * ld + kleft);
-#pragma unroll
-      for (int i = 0; i < R / 32; ++i) dma(rs, lane_off + (int)(32 * i * ld * 2), dst + (4 * i + wave) * 512);
+struct TileDma {
+  i32x4 r0, r1;    // r1: the up rows
+  int off, step;   // the lane's byte offset in instruction 0, bytes between instructions
+  uint32_t dst;
+
+  // the tile at row0, k0 of X; k0 >= K: an empty range, all zeros
+  __device__ __forceinline__ void at(const uint16_t* __restrict__ X, int64_t ld, int rows, int K, int row0, int k0,
+                                     uint32_t lds, int wave, int lane) {
+    const int kleft = max(K - k0, 0);
+    dst = lds + wave * 1024;
+    if constexpr (KMAJ) {
+      const int row = 8 * wave + (lane >> 3);  // + 32 i
+      const int c = (lane & 7) ^ ((row >> 1) & 7);
+      const int nr = min(rows - row0, GATED ? R / 2 : R);
+      const int64_t range = kleft > 0 ? (nr - 1) * ld + kleft : 0;
+      off = 8 * c < kleft ? (int)((row * ld + 8 * c) * 2) : kOut;
+      r0 = rsrc(X + row0 * ld + k0, range);
+      if constexpr (GATED) r1 = rsrc(X + (rows + row0) * ld + k0, range);
+      step = (int)(64 * ld);
     } else {
-      constexpr int GH = R / 4;
-      const int nr = min(rows - r0, R / 2);
-      const auto rg = rsrc(X + r0 * ld + k0, (nr - 1) * ld + kleft);
-      const auto ru = rsrc(X + (rows + r0) * ld + k0, (nr - 1) * ld + kleft);
-#pragma unroll
-      for (int i = 0; i < R / 32; ++i) {
-        const int grp = 32 * i / GH, at = (grp >> 1) * GH + 32 * i % GH;
-        dma(grp & 1 ? ru : rg, lane_off + (int)(at * ld * 2), dst + (4 * i + wave) * 512);
-      }
+      constexpr int LPR = R / 8, KPI = 64 / LPR;  // lanes per k row, k rows per instruction
+      const int kr = KPI * wave + lane / LPR;      // + 4 KPI i
+      const int c = (lane % LPR) ^ ((kr & 3) << 1);
+      // chunks past the last row would run into the next k row; their outputs are not stored
+      off = 8 * c < rows - row0 ? (int)((kr * ld + 8 * c) * 2) : kOut;
+      r0 = rsrc(X + k0 * ld + row0, kleft > 0 ? (min(kleft, BK) - 1) * ld + (rows - row0) : 0);
+      step = (int)(8 * KPI * ld);
     }
-  } else {
-    constexpr int LPR = R / 8;              // lanes per k row
-    constexpr int KPI = 64 / LPR;           // k rows per wave instruction
-    const int kr = KPI * wave + lane / LPR;  // + 4 KPI i
-    const int c = (lane % LPR) ^ ((kr & 3) << 1);
-    const int nk = min(kleft, BK);
-    const auto rs = rsrc(X + k0 * ld + r0, (nk - 1) * ld + (rows - r0));
-    // a last tile narrower than R: chunks past its rows would run into the next k row; they are read as
-    // zeros (their outputs are not stored)
-    const int lane_off = 8 * c < rows - r0 ? (int)((kr * ld + 8 * c) * 2) : kOut;
-#pragma unroll
-    for (int i = 0; i < BK / (4 * KPI); ++i)
-      dma(rs, lane_off + (int)(4 * KPI * i * ld * 2), dst + (4 * i + wave) * 512);
   }
-}
+  __device__ __forceinline__ void issue(int i) const {
+    if constexpr (GATED) {
+      constexpr int GH = R / 4;
+      const int grp = 32 * i / GH, row = (grp >> 1) * GH + 32 * i % GH;
+      dma(grp & 1 ? r1 : r0, off + row / 32 * step, dst + i * 4096);
+    } else {
+      dma(r0, off + i * step, dst + i * 4096);
+    }
+  }
+};
 
 // fragment of 32 rows at k step kk (16 deep): lane l holds row rowbase + (l & 31), k = 16 kk + 8 (l >> 5) + j
 template <bool KMAJ, int R>
@@ -203,15 +218,24 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
   const int tiles_m = (P.M + BM - 1) / BM, tiles_n = (P.N + HN - 1) / HN;
   int bm, bn;
   tile_coords(tiles_m, tiles_n, bm, bn);
-  const int row0 = bm * BM, col0 = bn * HN;
+  // in scalar registers for certain (the divisions above run on the vector unit): the DMA's ranges need it
+  const int row0 = __builtin_amdgcn_readfirstlane(bm * BM), col0 = __builtin_amdgcn_readfirstlane(bn * HN);
   const int kbeg = (int)blockIdx.y * P.kchunk, kend = min(P.K, kbeg + P.kchunk);
   const int nk = (kend - kbeg + BK - 1) / BK;
 
+  const uint32_t lds0 = lds_addr(lds);
   auto a_buf = [&](int b) { return lds + b * (TA + TB); };
   auto b_buf = [&](int b) { return lds + b * (TA + TB) + TA; };
-  auto issue = [&](int kt, int b) {
-    issue_tile<AK, BM, false>(P.A, P.lda, P.M, kend, row0, kbeg + kt * BK, a_buf(b), wave, lane);
-    issue_tile<BKM, BN, OP == kFfnGated>(P.B, P.ldb, P.N, kend, col0, kbeg + kt * BK, b_buf(b), wave, lane);
+  constexpr int DA = BM / 32, DMAS = DA + BN / 32;  // DMA instructions of a tile: A's, then B's
+  TileDma<AK, BM, false> ta;
+  TileDma<BKM, BN, OP == kFfnGated> tb;
+  auto aim = [&](int kt, int b) {
+    ta.at(P.A, P.lda, P.M, kend, row0, kbeg + kt * BK, lds0 + b * (TA + TB) * 2, wave, lane);
+    tb.at(P.B, P.ldb, P.N, kend, col0, kbeg + kt * BK, lds0 + (b * (TA + TB) + TA) * 2, wave, lane);
+  };
+  auto issue = [&](int i) {
+    if (i < DA) ta.issue(i);
+    else tb.issue(i - DA);
   };
 
   f32x16 acc[4][NJ];
@@ -220,41 +244,57 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = mfma::zero16();
   s16x8 fa[2][4], fb[2][NJ];
-  auto read = [&](int b, int kk, int set) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fa[set][i] = frag<AK, BM>(a_buf(b), wm * 128 + 32 * i, kk, lane);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) fb[set][j] = frag<BKM, BN>(b_buf(b), wn * (BN / 2) + 32 * j, kk, lane);
+  constexpr int FRAGS = 4 + NJ, MFMAS = 4 * NJ;
+  auto read = [&](int f, int b, int kk, int set) {  // fragment f of a step: B's, then A's
+    if (f < NJ) fb[set][f] = frag<BKM, BN>(b_buf(b), wn * (BN / 2) + 32 * f, kk, lane);
+    else fa[set][f - NJ] = frag<AK, BM>(a_buf(b), wm * 128 + 32 * (f - NJ), kk, lane);
   };
-  auto mma = [&](int set) {
+  // One k step: MFMA by MFMA, each with its share of the reads of the next step's fragments (in the first
+  // half of the step) and of the DMA (in the second); the order is pinned, since the compiler sinks the
+  // reads to just before their MFMAs and the wave then waits out every one of them.
+  auto step = [&](int set, int b, int kk, auto with_dma) {
+    constexpr bool DMA = decltype(with_dma)::value;
+    constexpr int H = MFMAS / 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int m = 0; m < MFMAS; ++m) {
+      acc[m / NJ][m % NJ] = mfma::mma<T>(fb[set][m % NJ], fa[set][m / NJ], acc[m / NJ][m % NJ]);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = mfma::mma<T>(fb[set][j], fa[set][i], acc[i][j]);
+      for (int f = 0; f < FRAGS; ++f)
+        if (f * H / FRAGS == m) read(f, b, kk, set ^ 1);
+      if constexpr (DMA) {
+#pragma unroll
+        for (int i = 0; i < DMAS; ++i)
+          if (H + i * H / DMAS == m) issue(i);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
-  issue(0, 0);
+  aim(0, 0);
+#pragma unroll
+  for (int i = 0; i < DMAS; ++i) issue(i);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (nk > 1) issue(1, 1);
-  read(0, 0, 0);
+  aim(1, 1);
+#pragma unroll
+  for (int i = 0; i < DMAS; ++i) issue(i);
+#pragma unroll
+  for (int f = 0; f < FRAGS; ++f) read(f, 0, 0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  // the DMA of tiles past the last one (empty range: zeros) and the last tile's read-ahead run like the
+  // others: no branch splits the schedule
   for (int kt = 0; kt < nk; ++kt) {
     const int cur = kt & 1;
-    read(cur, 1, 1);
-    mma(0);
-    read(cur, 2, 0);
-    mma(1);
-    read(cur, 3, 1);
-    mma(0);
-    if (kt + 1 < nk) {
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (kt + 2 < nk) issue(kt + 2, cur);
-      read(cur ^ 1, 0, 0);
-    }
-    mma(1);
+    step(0, cur, 1, std::false_type{});
+    step(1, cur, 2, std::false_type{});
+    step(0, cur, 3, std::false_type{});
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    aim(kt + 2, cur);
+    step(1, cur ^ 1, 0, std::true_type{});
   }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
 
   // ---- epilogue; lane: row 32 i + (lane & 31) of the wave, columns 32 j + 8 q + 4 (lane >> 5) + 0..3 ----
