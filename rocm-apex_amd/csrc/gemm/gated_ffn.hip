@@ -13,11 +13,11 @@
 // tile is on its way by LDS-DMA.  One barrier per K tile:
 //
 //   k step 0..2 of tile t : read step + 1's fragments, 4 x NJ MFMAs
-//   k step 3              : all reads of tile t are done, tile t + 1 has landed; barrier; start the DMA of
-//                           tile t + 2 into tile t's buffer, read tile t + 1's step 0, MFMAs
+//   k step 3              : all reads of tile t are done, tile t + 1 has landed; barrier; tile t's LDS goes
+//                           to the DMA of later tiles (Ring), read tile t + 1's step 0, MFMAs
 //
-// so a DMA has four k steps (about 2000 cycles) to land.  Operand tiles come through buffer loads whose
-// range ends at the matrix: rows, k steps past an edge arrive as zeros, no K multiple is needed.
+// Operand tiles come through buffer loads whose range ends at the matrix: rows and k steps past an edge
+// arrive as zeros, no K multiple is needed.
 //
 // The gate and up columns of a tile are dealt so that a wave holds both for the same outputs (its
 // first BN/4 columns are rows of Wg, its last BN/4 the same rows of Wu): act(a) u is taken on the
@@ -200,9 +200,69 @@ __device__ __forceinline__ void store_image(const uint16_t* img, T* C, int64_t l
   }
 }
 
+// The LDS ring of operand tiles (byte offsets).
+// BN = 256: five 32-KB slots, A and B tiles in turn (A(t) in slot 2t mod 5, B(t) in 2t + 1 mod 5).  When tile
+// t has been read, B(t + 2) goes into A(t)'s slot and A(t + 3) into B(t)'s: B has three k steps to land,
+// A seven.  Two buffers of both, the DMA of a whole tile in its predecessor's last step, left the
+// MFMAs waiting 45 % of the time.
+// BN = 128: three slots of A and B; tile t + 3 replaces tile t.
+// kFirst of a round's instructions (B's, then A's) go out in the step after the barrier, the others in the
+// next two steps.  kInFlight: instructions younger than tile t + 1's at the barrier that opens it.
+template <int BN> struct Ring;
+template <> struct Ring<256> {
+  static constexpr int kSlot = 32768, kBytes = 5 * kSlot;
+  static constexpr int kFirst = 8, kAheadB = 2, kInFlight = 8, kAfterPrologue = 16;
+  static __device__ constexpr int first_a() { return 0; }
+  static __device__ constexpr int first_b() { return kSlot; }
+  static __device__ __forceinline__ int next_b_slot(int sa, int) { return sa; }
+  static __device__ __forceinline__ int next_a_slot(int, int sb) { return sb; }
+  static __device__ __forceinline__ void advance(int& sa, int& sb) {
+    sa = sa + 2 * kSlot >= kBytes ? sa + 2 * kSlot - kBytes : sa + 2 * kSlot;
+    sb = sa + kSlot >= kBytes ? sa + kSlot - kBytes : sa + kSlot;
+  }
+  // A0 B0 A1, and B1 of the round (B1, A2)
+  template <int DA, int DB, typename AA, typename AB, typename IA, typename IB>
+  static __device__ __forceinline__ void prologue(AA aim_a, AB aim_b, IA issue_a, IB issue_b) {
+    aim_a(0, 0);
+    for (int i = 0; i < DA; ++i) issue_a(i);
+    aim_b(0, kSlot);
+    for (int i = 0; i < DB; ++i) issue_b(i);
+    aim_a(1, 2 * kSlot);
+    for (int i = 0; i < DA; ++i) issue_a(i);
+    aim_b(1, 3 * kSlot);
+    for (int i = 0; i < DB; ++i) issue_b(i);
+    aim_a(2, 4 * kSlot);
+  }
+};
+template <> struct Ring<128> {
+  static constexpr int kA = 32768, kSlot = 49152, kBytes = 3 * kSlot;
+  static constexpr int kFirst = 4, kAheadB = 3, kInFlight = 12, kAfterPrologue = 16;
+  static __device__ constexpr int first_a() { return 0; }
+  static __device__ constexpr int first_b() { return kA; }
+  static __device__ __forceinline__ int next_b_slot(int, int sb) { return sb; }
+  static __device__ __forceinline__ int next_a_slot(int sa, int) { return sa; }
+  static __device__ __forceinline__ void advance(int& sa, int& sb) {
+    sa = sa + kSlot >= kBytes ? 0 : sa + kSlot;
+    sb = sa + kA;
+  }
+  // tiles 0 and 1, and B2 of the round (B2, A2)
+  template <int DA, int DB, typename AA, typename AB, typename IA, typename IB>
+  static __device__ __forceinline__ void prologue(AA aim_a, AB aim_b, IA issue_a, IB issue_b) {
+    for (int t = 0; t < 2; ++t) {
+      aim_b(t, t * kSlot + kA);
+      for (int i = 0; i < DB; ++i) issue_b(i);
+      aim_a(t, t * kSlot);
+      for (int i = 0; i < DA; ++i) issue_a(i);
+    }
+    aim_b(2, 2 * kSlot + kA);
+    for (int i = 0; i < DB; ++i) issue_b(i);
+    aim_a(2, 2 * kSlot);
+  }
+};
+
 template <int BN, int OP>
 constexpr size_t lds_bytes() {
-  const size_t ops = (size_t)2 * (BM + BN) * BK * 2;
+  const size_t ops = Ring<BN>::kBytes;
   const size_t epi = OP == kFfnDGated ? (size_t)128 * (BN + 4) * 4 : (size_t)BM * (BN + 8) * 2;
   return ops > epi ? ops : epi;
 }
@@ -211,7 +271,6 @@ template <typename T, bool AK, bool BKM, int OP, int BN, int ACT>
 __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
   constexpr int NJ = BN / 64;                    // 32-column fragments per wave
   constexpr int HN = OP == kFfnGated ? BN / 2 : BN;  // output columns per tile
-  constexpr int TA = BM * BK, TB = BN * BK;
   extern __shared__ __attribute__((aligned(16))) uint16_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -223,19 +282,21 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
   const int kbeg = (int)blockIdx.y * P.kchunk, kend = min(P.K, kbeg + P.kchunk);
   const int nk = (kend - kbeg + BK - 1) / BK;
 
+  using R = Ring<BN>;
+  constexpr int DA = BM / 32, DB = BN / 32;  // DMA instructions of an A and a B tile
   const uint32_t lds0 = lds_addr(lds);
-  auto a_buf = [&](int b) { return lds + b * (TA + TB); };
-  auto b_buf = [&](int b) { return lds + b * (TA + TB) + TA; };
-  constexpr int DA = BM / 32, DMAS = DA + BN / 32;  // DMA instructions of a tile: A's, then B's
   TileDma<AK, BM, false> ta;
   TileDma<BKM, BN, OP == kFfnGated> tb;
-  auto aim = [&](int kt, int b) {
-    ta.at(P.A, P.lda, P.M, kend, row0, kbeg + kt * BK, lds0 + b * (TA + TB) * 2, wave, lane);
-    tb.at(P.B, P.ldb, P.N, kend, col0, kbeg + kt * BK, lds0 + (b * (TA + TB) + TA) * 2, wave, lane);
+  auto aim_a = [&](int kt, int slot) {
+    ta.at(P.A, P.lda, P.M, kend, row0, kbeg + kt * BK, lds0 + slot, wave, lane);
   };
+  auto aim_b = [&](int kt, int slot) {
+    tb.at(P.B, P.ldb, P.N, kend, col0, kbeg + kt * BK, lds0 + slot, wave, lane);
+  };
+  // DMA of one round: B's instructions, then A's
   auto issue = [&](int i) {
-    if (i < DA) ta.issue(i);
-    else tb.issue(i - DA);
+    if (i < DB) tb.issue(i);
+    else ta.issue(i - DB);
   };
 
   f32x16 acc[4][NJ];
@@ -245,54 +306,59 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
     for (int j = 0; j < NJ; ++j) acc[i][j] = mfma::zero16();
   s16x8 fa[2][4], fb[2][NJ];
   constexpr int FRAGS = 4 + NJ, MFMAS = 4 * NJ;
-  auto read = [&](int f, int b, int kk, int set) {  // fragment f of a step: B's, then A's
-    if (f < NJ) fb[set][f] = frag<BKM, BN>(b_buf(b), wn * (BN / 2) + 32 * f, kk, lane);
-    else fa[set][f - NJ] = frag<AK, BM>(a_buf(b), wm * 128 + 32 * (f - NJ), kk, lane);
+  const uint16_t *at, *bt;  // the tile that is read
+  auto read = [&](int f, int kk, int set) {  // fragment f of a step: B's, then A's
+    if (f < NJ) fb[set][f] = frag<BKM, BN>(bt, wn * (BN / 2) + 32 * f, kk, lane);
+    else fa[set][f - NJ] = frag<AK, BM>(at, wm * 128 + 32 * (f - NJ), kk, lane);
   };
   // One k step: MFMA by MFMA, each with its share of the reads of the next step's fragments (in the first
-  // half of the step) and of the DMA (in the second); the order is pinned, since the compiler sinks the
-  // reads to just before their MFMAs and the wave then waits out every one of them.
-  auto step = [&](int set, int b, int kk, auto with_dma) {
-    constexpr bool DMA = decltype(with_dma)::value;
-    constexpr int H = MFMAS / 2;
+  // half of the step) and of DMA instructions D0 .. D1 - 1 (evenly: more at once than the CU's address
+  // unit takes, 16 cycles each, would hold up the MFMAs behind them).  The order is pinned, since the
+  // compiler sinks the reads to just before their MFMAs and the wave then waits out every one of them.
+  auto step = [&](int set, int kk, auto d0, auto d1) {
+    constexpr int H = MFMAS / 2, D0 = decltype(d0)::value, D1 = decltype(d1)::value;
 #pragma unroll
     for (int m = 0; m < MFMAS; ++m) {
       acc[m / NJ][m % NJ] = mfma::mma<T>(fb[set][m % NJ], fa[set][m / NJ], acc[m / NJ][m % NJ]);
 #pragma unroll
       for (int f = 0; f < FRAGS; ++f)
-        if (f * H / FRAGS == m) read(f, b, kk, set ^ 1);
-      if constexpr (DMA) {
+        if (f * H / FRAGS == m) read(f, kk, set ^ 1);
 #pragma unroll
-        for (int i = 0; i < DMAS; ++i)
-          if (H + i * H / DMAS == m) issue(i);
-      }
+      for (int i = D0; i < D1; ++i)
+        if ((i - D0) * MFMAS / (D1 - D0) == m) issue(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  using Zero = std::integral_constant<int, 0>;
+  using First = std::integral_constant<int, R::kFirst>;
+  using Half = std::integral_constant<int, (R::kFirst + DA + DB) / 2>;
+  using All = std::integral_constant<int, DA + DB>;
 
-  aim(0, 0);
-#pragma unroll
-  for (int i = 0; i < DMAS; ++i) issue(i);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // Before tile 0: the tiles and the first part of the round that tile -1's last step would have issued
+  int sa = R::first_a(), sb = R::first_b();  // slots of the current tile
+  R::template prologue<DA, DB>(aim_a, aim_b, [&](int i) { ta.issue(i); }, [&](int i) { tb.issue(i); });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R::kAfterPrologue) : "memory");
   __syncthreads();
-  aim(1, 1);
+  at = lds + sa / 2;
+  bt = lds + sb / 2;
 #pragma unroll
-  for (int i = 0; i < DMAS; ++i) issue(i);
-#pragma unroll
-  for (int f = 0; f < FRAGS; ++f) read(f, 0, 0, 0);
+  for (int f = 0; f < FRAGS; ++f) read(f, 0, 0);
   __builtin_amdgcn_sched_barrier(0);
   // the DMA of tiles past the last one (empty range: zeros) and the last tile's read-ahead run like the
   // others: no branch splits the schedule
   for (int kt = 0; kt < nk; ++kt) {
-    const int cur = kt & 1;
-    step(0, cur, 1, std::false_type{});
-    step(1, cur, 2, std::false_type{});
-    step(0, cur, 3, std::false_type{});
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    step(0, 1, First{}, Half{});
+    step(1, 2, Half{}, All{});
+    step(0, 3, Zero{}, Zero{});
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(R::kInFlight) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    aim(kt + 2, cur);
-    step(1, cur ^ 1, 0, std::true_type{});
+    aim_b(kt + R::kAheadB, R::next_b_slot(sa, sb));
+    aim_a(kt + 3, R::next_a_slot(sa, sb));
+    R::advance(sa, sb);
+    at = lds + sa / 2;
+    bt = lds + sb / 2;
+    step(1, 0, Zero{}, First{});
   }
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
