@@ -498,6 +498,134 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// Few rows (a token each of up to 32 sequences): the weights are read once and nothing else counts.
+// A workgroup owns 16 outputs (16 rows of Wg and of Wu, or of W2) and its NW waves split K; the weights
+// go straight from memory to the MFMA operand (16 rows x 32 k a load), U steps in flight per wave, x comes
+// from the caches.  The waves' partial tiles meet in LDS in a fixed order, where the block's
+// epilogue (bias, activation, product) runs in fp32.
+// ---------------------------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(i32x4 a, i32x4 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mma16<bf16_t>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mfma::bf16x8, a),
+                                                 __builtin_bit_cast(mfma::bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<f16_t>(i32x4 a, i32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mfma::f16x8, a), __builtin_bit_cast(mfma::f16x8, b),
+                                                c, 0, 0, 0);
+}
+
+constexpr int kFewRows = 32;
+
+template <typename T, bool GATED, int ACT, int TM, int NW>
+__global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
+  constexpr int G = GATED ? 2 : 1, U = TM == 1 && !GATED ? 8 : 4;
+  constexpr int TP = 16 * G + 4;  // floats a token takes in a wave's partial tile
+  extern __shared__ __attribute__((aligned(16))) float part[];  // [NW][16 TM][TP]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int col0 = blockIdx.x * 16, l16 = lane & 15, g8 = 8 * (lane >> 4);
+  const int chunk = ((P.K + NW - 1) / NW + 31) / 32 * 32;
+  const int k1 = min(P.K, (wave + 1) * chunk);
+  int k = wave * chunk;
+
+  // buffer ranges end at the last row and K's end: loads past them give zeros
+  const int rows = min(16, P.N - col0);
+  __amdgpu_buffer_rsrc_t rw[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+    rw[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(P.B + ((int64_t)g * P.N + col0) * P.ldb), 0,
+                                              (int)(((rows - 1) * P.ldb + P.K) * 2), 0x00027000);
+  const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)P.A, 0, (int)(((P.M - 1) * P.lda + P.K) * 2), 0x00027000);
+  const int ow = (int)((l16 * P.ldb + g8) * 2);
+  int ox[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) ox[t] = (int)(((16 * t + l16) * P.lda + g8) * 2);
+  f32x4 acc[G][TM];
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int t = 0; t < TM; ++t) acc[g][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // U steps of loads, all in flight, then their MFMAs; the last group's loads past the wave's chunk are zeros
+  auto group = [&](auto last) {
+    i32x4 wv[U][G], xv[U][TM];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = !decltype(last)::value || k + 32 * u + g8 < k1;
+      const int at = 2 * (k + 32 * u);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        wv[u][g] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[g], in ? ow + at : kOut, 0, 0));
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+        xv[u][t] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, in ? ox[t] + at : kOut, 0, 0));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) acc[g][t] = mma16<T>(wv[u][g], xv[u][t], acc[g][t]);
+  };
+  for (; k + 32 * U <= k1; k += 32 * U) group(std::false_type{});
+  if (k < k1) group(std::true_type{});
+  // lane: token 16 t + (lane & 15), outputs 4 (lane >> 4) + 0..3
+#pragma unroll
+  for (int t = 0; t < TM; ++t)
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      *reinterpret_cast<f32x4*>(part + ((wave * TM + t) * 16 + l16) * TP + 16 * g + 4 * (lane >> 4)) = acc[g][t];
+  __syncthreads();
+  for (int i = tid; i < P.M * 16; i += NW * 64) {
+    const int tok = i >> 4, c = i & 15, gc = col0 + c;
+    if (gc >= P.N) continue;
+    float v[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < NW; ++q) s += part[(q * TM * 16 + tok) * TP + 16 * g + c];
+      v[g] = s + (P.bias != nullptr ? to_f(((const T*)P.bias)[(int64_t)g * P.N + gc]) : 0.f);
+    }
+    if constexpr (GATED) {
+      if (P.aux_out != nullptr) {
+        T* au = (T*)P.aux_out + (int64_t)tok * 2 * P.N + gc;
+        au[0] = from_f<T>(v[0]);
+        au[P.N] = from_f<T>(v[1]);
+      }
+      float d;
+      v[0] = activate<ACT>(v[0], d) * v[1];
+    }
+    ((T*)P.C)[(int64_t)tok * P.ldc + gc] = from_f<T>(v[0]);
+  }
+}
+
+template <typename T, bool GATED, int ACT, int TM, int NW>
+void launch_few(const FfnArgs& g, hipStream_t s) {
+  Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.aux_in,
+           g.aux_out, nullptr, g.k};
+  const size_t lds = (size_t)NW * TM * 16 * (16 * (GATED ? 2 : 1) + 4) * sizeof(float);
+  hipLaunchKernelGGL((ffn_few_kernel<T, GATED, ACT, TM, NW>), dim3((unsigned)((g.n + 15) / 16)), dim3(NW * 64), lds, s, P);
+}
+
+// 16 waves a workgroup where there are too few outputs for two workgroups a CU, else 8
+template <typename T, bool GATED, int ACT>
+void launch_few_tm(const FfnArgs& g, int cus, hipStream_t s) {
+  const bool wide = (g.n + 15) / 16 < 2 * cus;
+  auto go = [&](auto tm) {
+    constexpr int TM = decltype(tm)::value;
+    if (wide) launch_few<T, GATED, ACT, TM, 16>(g, s);
+    else launch_few<T, GATED, ACT, TM, 8>(g, s);
+  };
+  if (g.m <= 16) go(std::integral_constant<int, 1>{});
+  else go(std::integral_constant<int, 2>{});
+}
+
 // sum of the split-K partials (fixed order) + bias
 template <typename T>
 __global__ void __launch_bounds__(256) ffn_reduce(const float* __restrict__ part, int splits, int64_t M, int N,
@@ -598,13 +726,27 @@ bool ffn_supported(const FfnArgs& g) {
   }
 }
 
+// up to 32 rows of a k-major x k-major product
+static bool ffn_few(const FfnArgs& g) { return g.m <= ffn::kFewRows && g.a_kmajor && g.b_kmajor; }
+
 int64_t ffn_workspace_floats(const FfnArgs& g, int cus) {
+  if (ffn_few(g)) return 0;
   const ffn::Plan p = ffn::make_plan(g, cus);
   return p.splits > 1 ? (int64_t)p.splits * g.m * g.n : 0;
 }
 
 void ffn_gemm(const FfnArgs& g, int cus, hipStream_t s) {
   if (!ffn_supported(g)) throw std::runtime_error("gated_ffn: unsupported shape, alignment or dtype");
+  if (ffn_few(g)) {
+    dispatch_16(g.dtype, [&](auto tag) {
+      using T = typename decltype(tag)::type;
+      if (g.op != kFfnGated) ffn::launch_few_tm<T, false, 0>(g, cus, s);
+      else if (g.act == kGateSilu) ffn::launch_few_tm<T, true, kGateSilu>(g, cus, s);
+      else ffn::launch_few_tm<T, true, kGateGelu>(g, cus, s);
+    }, "gated_ffn");
+    check_launch("gated_ffn");
+    return;
+  }
   const ffn::Plan p = ffn::make_plan(g, cus);
   if (p.splits > 1 && g.ws == nullptr) throw std::runtime_error("gated_ffn: workspace missing");
   dispatch_16(g.dtype, [&](auto tag) {
