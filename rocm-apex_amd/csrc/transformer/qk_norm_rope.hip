@@ -17,7 +17,6 @@
 // dw: fp32 per lane over the persistent loop, per block through LDS, then a fixed-order column sum
 // over the blocks (no atomics: the same inputs give the same bits).
 // Positions outside the table give NaN rows (the table is never read past its end).
-#include "apex_amd/colreduce.h"
 #include "apex_amd/device.h"
 #include "apex_amd/dispatch.h"
 #include "apex_amd/qk_norm_rope_api.h"
@@ -279,14 +278,30 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
   }
 }
 
-// dw[c] = sum over a side's blocks, fixed order; blockIdx.y = 0: q, 1: k
+// dw[c] = sum over a side's blocks, fixed order; blockIdx.y = 0: q, 1: k.  16 columns x 64 row groups a
+// block: a column is a chain of parts / 64 / 4 loads (a thousand parts, 16 groups: 14 us, 64: 5)
 template <typename TW>
-__global__ void __launch_bounds__(256) dw_finalize(const float* __restrict__ part, int bq, int bk, int d, TW* dq, TW* dk) {
-  __shared__ float red[16][17];
+__global__ void __launch_bounds__(1024) dw_finalize(const float* __restrict__ part, int bq, int bk, int d, TW* dq, TW* dk) {
+  __shared__ float red[64][17];
   const bool isk = blockIdx.y != 0;
-  const float v = colreduce16(part + (isk ? (int64_t)bq * d : 0), isk ? bk : bq, d, red);
-  const int c = blockIdx.x * 16 + (threadIdx.x & 15);
-  if ((threadIdx.x >> 4) == 0 && c < d) (isk ? dk : dq)[c] = from_f<TW>(v);
+  const float* p = part + (isk ? (int64_t)bq * d : 0);
+  const int parts = isk ? bk : bq, cl = threadIdx.x & 15, grp = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  if (c < d) {
+    int j = grp;
+    for (; j + 192 < parts; j += 256) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a[u] += p[(int64_t)(j + 64 * u) * d + c];
+    }
+    for (; j < parts; j += 64) a[0] += p[(int64_t)j * d + c];
+  }
+  red[grp][cl] = (a[0] + a[1]) + (a[2] + a[3]);
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (grp < o) red[grp][cl] += red[grp + o][cl];
+    __syncthreads();
+  }
+  if (grp == 0 && c < d) (isk ? dk : dq)[c] = from_f<TW>(red[0][cl]);
 }
 
 struct Plan {
@@ -313,7 +328,7 @@ inline Plan make_plan(const QkRopeArgs& a, int cus, bool bwd) {
   const int64_t rows = tokens * (a.hq + a.hk);
   p.hb = rows >= (int64_t)cus * groups * 4 ? (bwd ? 2 : 4) : 1;
   const int heads[2] = {a.hq, a.hk};
-  int64_t cap = (int64_t)cus * 8;
+  int64_t cap = (int64_t)cus * 8;  // persistent; four a CU made the backward 257 us at 32768 x 40 x 128 (222)
   for (int i = 0; i < 2; ++i) {
     p.sub[i] = (heads[i] + p.hb - 1) / p.hb;
     const int64_t need = (tokens * p.sub[i] + groups - 1) / groups;
@@ -350,7 +365,7 @@ void launch(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
   hipLaunchKernelGGL((qk_kernel<T, TW, PV, NJ, HB, INTER, BWD, WEIGHT>), dim3(p.blocks[0] + p.blocks[1]),
                      dim3(kThreads), lds, s, P, p.g);
   if (BWD && WEIGHT)
-    hipLaunchKernelGGL((dw_finalize<TW>), dim3((a.d + 15) / 16, 2), dim3(256), 0, s, a.part, p.blocks[0], p.blocks[1],
+    hipLaunchKernelGGL((dw_finalize<TW>), dim3((a.d + 15) / 16, 2), dim3(1024), 0, s, a.part, p.blocks[0], p.blocks[1],
                        a.d, (TW*)a.dqw, (TW*)a.dkw);
 }
 

@@ -72,23 +72,28 @@ __device__ __forceinline__ void accumulate(float& m, float& s, const float (&x)[
   m = M;
 }
 
-// Teacher weights of a row into LDS: cls[k] (-1: none) and t[k]; also log2 t in lt (forward).
-// Returns the row's state in every thread: 0 no entries, 1 usable, 2 a class past the vocabulary.
-// All threads call it; `red` holds 2 * kWaves floats.
+// The row's teacher entries into LDS: class (-1: none) and logit.  Returns the row's state in every thread:
+// 0 no entries (or all -inf), 1 usable, 2 a class past the vocabulary.  All threads call it and the two
+// below; `red` holds 2 * kWaves floats.
 template <typename TI>
-__device__ __forceinline__ int teacher_row(const float* __restrict__ z, const TI* __restrict__ idx, int top, int classes,
-                                           float c, int* cls, float* t, float* lt, float* red) {
-  float m = -INFINITY;
-  int state = 0;
+__device__ __forceinline__ int teacher_entries(const float* __restrict__ z, const TI* __restrict__ idx, int top,
+                                               int classes, int* cls, float* t, float* red) {
+  float state = 0.f;
   for (int k = threadIdx.x; k < top; k += kThreads) {
     const int64_t j = (int64_t)idx[k];
     const bool in = j >= 0 && j < classes;
-    if (j >= 0) state |= in ? 1 : 2;
     const float y = in ? z[k] : -INFINITY;
     cls[k] = in ? (int)j : -1;
     t[k] = y;
-    m = fmaxf(m, y);
+    state = fmaxf(state, j >= classes ? 2.f : y != -INFINITY ? 1.f : 0.f);
   }
+  return (int)block_max(state, red);
+}
+
+// logits in t -> weights; log2 of them in lt (forward)
+__device__ __forceinline__ void teacher_weights(int top, float c, float* t, float* lt, float* red) {
+  float m = -INFINITY;
+  for (int k = threadIdx.x; k < top; k += kThreads) m = fmaxf(m, t[k]);
   m = block_max(m, red);
   const float b = base(m);
   float s = 0.f;
@@ -98,10 +103,9 @@ __device__ __forceinline__ int teacher_row(const float* __restrict__ z, const TI
   for (int k = threadIdx.x; k < top; k += kThreads) {
     const float y = (t[k] - b) * c;
     if (lt != nullptr) lt[k] = y - ls;
-    t[k] = s == 0.f ? 0.f : exp2_(y) * inv;
+    t[k] = exp2_(y) * inv;
   }
-  const int any = __syncthreads_or(state & 1), bad = __syncthreads_or(state & 2);
-  return bad ? 2 : (any && s != 0.f) ? 1 : 0;
+  __syncthreads();
 }
 
 // the row's loss and its (maximum, sum), from the latter (thread 0 writes)
@@ -134,12 +138,17 @@ kd_fwd_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const fl
   const int c0 = blockIdx.y * chunk, c1 = min(classes, c0 + chunk);
   float m = -INFINITY, s = 0.f;
   int v = c0 + threadIdx.x * 8;
-  for (; v + 8 * kThreads + 8 <= c1; v += 16 * kThreads) {  // two vectors in flight
-    float r0[8], r1[8];
-    load8<T>(r0, x + v);
-    load8<T>(r1, x + v + 8 * kThreads);
-    accumulate<8>(m, s, r0, c);
-    accumulate<8>(m, s, r1, c);
+  for (; v + 24 * kThreads + 8 <= c1; v += 32 * kThreads) {  // four vectors in flight
+    Pack8<T> w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const Pack8<T>*>(x + v + 8 * kThreads * i);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float r[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] = to_f(w[i].e[k]);
+      accumulate<8>(m, s, r, c);
+    }
   }
   for (; v + 8 <= c1; v += 8 * kThreads) {
     float r0[8];
@@ -168,7 +177,8 @@ kd_fwd_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const fl
   }
   int* cls = (int*)lds;
   float *t = lds + top, *lt = lds + 2 * top;
-  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, lt, red);
+  const int state = teacher_entries(tz + row * top, ti + row * top, top, classes, cls, t, red);
+  if (state == 1) teacher_weights(top, c, t, lt, red);
   row_loss(x, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
 }
 
@@ -190,7 +200,8 @@ kd_join_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const f
   for (int o = 32; o > 0; o >>= 1) merge(m, s, __shfl_xor(m, o, 64), __shfl_xor(s, o, 64), c);
   int* cls = (int*)lds;
   float *t = lds + top, *lt = lds + 2 * top;
-  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, lt, red);
+  const int state = teacher_entries(tz + row * top, ti + row * top, top, classes, cls, t, red);
+  if (state == 1) teacher_weights(top, c, t, lt, red);
   row_loss(logits + row * pitch, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
 }
 
@@ -205,9 +216,13 @@ kd_bwd_kernel(const float* __restrict__ gl, int64_t gl_stride, const T* __restri
   const T* x = logits + row * pitch;
   T* gx = grad + row * classes;
   const int c0 = blockIdx.y * chunk, c1 = min(classes, c0 + chunk);
+  // a lane's first vector is on its way while the teacher's entries are read
+  int v = c0 + threadIdx.x * 8;
+  Pack8<T> next;
+  if (v + 8 <= c1) next = *reinterpret_cast<const Pack8<T>*>(x + v);
   int* cls = (int*)lds;
   float* t = lds + top;
-  const int state = teacher_row(tz + row * top, ti + row * top, top, classes, c, cls, t, nullptr, red);
+  const int state = teacher_entries(tz + row * top, ti + row * top, top, classes, cls, t, red);
   const float2 st = stats[row];
   const float b = base(st.x);
   const float coef = state == 2 ? __builtin_nanf("") : gl[row * gl_stride] * temp;
@@ -215,19 +230,24 @@ kd_bwd_kernel(const float* __restrict__ gl, int64_t gl_stride, const T* __restri
   const int tail = c0 + ((c1 - c0) & ~7);
   if (state == 0) {  // no teacher: a zero row whatever the logits and the incoming gradient hold
     const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int v = c0 + threadIdx.x * 8; v + 8 <= c1; v += 8 * kThreads) store8<T>(gx + v, zero);
+    for (; v + 8 <= c1; v += 8 * kThreads) store8<T>(gx + v, zero);
     for (int e = tail + threadIdx.x; e < c1; e += kThreads) gx[e] = from_f<T>(0.f);
     return;
   }
-  for (int v = c0 + threadIdx.x * 8; v + 8 <= c1; v += 8 * kThreads) {
+  for (; v + 8 <= c1; v += 8 * kThreads) {
+    const Pack8<T> w = next;
+    if (v + 8 * kThreads + 8 <= c1) next = *reinterpret_cast<const Pack8<T>*>(x + v + 8 * kThreads);
     float r[8];
-    load8<T>(r, x + v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) r[k] = to_f(w.e[k]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) r[k] = pc * exp2_((r[k] - b) * c);
     store8<T>(gx + v, r);
   }
   for (int e = tail + threadIdx.x; e < c1; e += kThreads) gx[e] = from_f<T>(pc * exp2_((to_f(x[e]) - b) * c));
-  __syncthreads();
+  if (state != 1) return;  // NaN everywhere already
+  // the weights are taken while the stores above drain; its barriers also order them before the stores below
+  teacher_weights(top, c, t, nullptr, red);
   for (int k = threadIdx.x; k < top; k += kThreads) {
     const int j = cls[k];
     if (j < c0 || j >= c1) continue;
@@ -242,10 +262,12 @@ kd_bwd_kernel(const float* __restrict__ gl, int64_t gl_stride, const T* __restri
   }
 }
 
-// parts of a row: one when the rows alone give every CU 4 workgroups, else enough for that, at
-// least 4096 classes each (16 vectors a lane... a shorter part is mostly launch and reduction)
-inline int row_parts(int64_t rows, int classes, int cus, int* chunk) {
-  int64_t p = rows >= (int64_t)cus * 4 ? 1 : ((int64_t)cus * 4 + rows - 1) / rows;
+// Parts of a row, of at least 4096 classes each.  Forward: one from two workgroups a CU on, else enough
+// for four (1021 rows of 50257 fp16: 22 us in one part, 25 in two with the join).  Backward, where a part
+// costs no join: enough for eight (the same rows: 51 us in one part, 45 in two).
+inline int row_parts(int64_t rows, int classes, int cus, bool bwd, int* chunk) {
+  const int64_t enough = (int64_t)cus * (bwd ? 8 : 2), target = (int64_t)cus * (bwd ? 8 : 4);
+  int64_t p = rows >= enough ? 1 : (target + rows - 1) / rows;
   const int64_t most = classes / 4096 > 1 ? classes / 4096 : 1;
   if (p > most) p = most;
   const int64_t each = ((int64_t)classes + p - 1) / p;
@@ -270,7 +292,7 @@ inline void check(const TopkDistillArgs& a) {
 
 int64_t topk_distill_part_floats(const TopkDistillArgs& a, int cus) {
   int chunk;
-  const int p = a.rows > 0 ? kd::row_parts(a.rows, a.classes, cus, &chunk) : 1;
+  const int p = a.rows > 0 ? kd::row_parts(a.rows, a.classes, cus, false, &chunk) : 1;
   return p > 1 ? 2 * a.rows * p : 0;
 }
 
@@ -278,7 +300,7 @@ void topk_distill_fwd(const TopkDistillArgs& a, float* losses, float* stats, flo
   kd::check(a);
   if (a.rows == 0) return;
   int chunk;
-  const int p = kd::row_parts(a.rows, a.classes, cus, &chunk);
+  const int p = kd::row_parts(a.rows, a.classes, cus, false, &chunk);
   const size_t lds = (size_t)3 * a.top * sizeof(float);
   const float c = 1.4426950408889634f / a.temperature;
   kd::dispatch(a, [&](auto tag, auto itag) {
@@ -300,7 +322,7 @@ void topk_distill_bwd(const TopkDistillArgs& a, const float* grad_loss, int64_t 
   kd::check(a);
   if (a.rows == 0) return;
   int chunk;
-  const int p = kd::row_parts(a.rows, a.classes, cus, &chunk);
+  const int p = kd::row_parts(a.rows, a.classes, cus, true, &chunk);
   const float c = 1.4426950408889634f / a.temperature;
   kd::dispatch(a, [&](auto tag, auto itag) {
     using T = typename decltype(tag)::type;
