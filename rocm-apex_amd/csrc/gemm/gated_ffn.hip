@@ -454,12 +454,23 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
     __syncthreads();
     store_image<T, HN, HP>(lds, (T*)P.C, P.ldc, row0, col0, P.M, P.N, tid);
   } else {
-    // dh stays fp32: 128 rows at a time through LDS, then 8 consecutive columns a thread with a and u
-    constexpr int CST = BN + 4, V = BN / 8, RPP = NT / V;
+    // dh stays fp32: 128 rows at a time through LDS, then 8 consecutive columns a thread with a and u.  These
+    // are fetched for all of a thread's rows of a half at once, the second half's into the registers
+    // that the first half's free (row by row, four at a time, their latency was a third of the kernel at
+    // 1024-deep products).
+    constexpr int CST = BN + 4, V = BN / 8, RPP = NT / V, IT = 128 / RPP;
     float* cs = reinterpret_cast<float*>(lds);
     const int ch = tid % V, gc = col0 + 8 * ch;
-    const T* au = (const T*)P.aux_in;
+    const T* au = (const T*)P.aux_in + min(gc, P.N - 8);  // clamped: loads past the edges are not used
     T* out = (T*)P.C;
+    uint4 pa[IT], pu[IT];
+    auto fetch = [&](int half, int it) {
+      const int64_t at = (int64_t)min(row0 + 128 * half + tid / V + RPP * it, P.M - 1) * P.ldc;
+      pa[it] = *reinterpret_cast<const uint4*>(au + at);
+      pu[it] = *reinterpret_cast<const uint4*>(au + at + P.N);
+    };
+#pragma unroll
+    for (int it = 0; it < IT; ++it) fetch(0, it);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (wm == half) {
@@ -473,24 +484,24 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
                   make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
       }
       __syncthreads();
-      if (gc < P.N) {
-#pragma unroll 4
-        for (int r = tid / V; r < 128; r += RPP) {
-          const int gr = row0 + 128 * half + r;
-          if (gr >= P.M) break;
-          const int64_t at = (int64_t)gr * P.ldc + gc;
-          float a[8], u[8], g[8], da[8], du[8];
-          Vec8<T>::load(a, au + at);
-          Vec8<T>::load(u, au + at + P.N);
-          Vec8<float>::load(g, cs + r * CST + 8 * ch);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float d;
-            du[e] = g[e] * activate<ACT>(a[e], d);
-            da[e] = g[e] * u[e] * d;
-          }
-          Vec8<T>::store(out + at, da);
-          Vec8<T>::store(out + at + P.N, du);
+      for (int it = 0; it < IT; ++it) {
+        const int r = tid / V + RPP * it, gr = row0 + 128 * half + r;
+        float a[8], u[8], g[8], da[8], du[8];
+        Vec8<T>::load(a, reinterpret_cast<const T*>(&pa[it]));
+        Vec8<T>::load(u, reinterpret_cast<const T*>(&pu[it]));
+        if (half == 0) fetch(1, it);
+        Vec8<float>::load(g, cs + r * CST + 8 * ch);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float d;
+          du[e] = g[e] * activate<ACT>(a[e], d);
+          da[e] = g[e] * u[e] * d;
+        }
+        if (gr < P.M && gc < P.N) {
+          T* o = out + (int64_t)gr * P.ldc + gc;
+          Vec8<T>::store(o, da);
+          Vec8<T>::store(o + P.N, du);
         }
       }
       __syncthreads();
