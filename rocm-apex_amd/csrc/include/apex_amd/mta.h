@@ -8,6 +8,7 @@
 // persistent, grid-strided kernel sized to the 256 CUs, and it is capturable in a hipGraph
 // (no per-call H2D copy once the table is cached).
 #pragma once
+#include <type_traits>
 #include "apex_amd/device.h"
 
 namespace apex_amd {
@@ -124,7 +125,19 @@ struct ListIO {
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::load_vec(r, base, i);
   }
   static __device__ __forceinline__ void store_vec(const float (&r)[D][kVec], void* const (&base)[D], int i) {
-    if constexpr ((Op::kWrite >> I) & 1u) MtaIO<T>::store(reinterpret_cast<T*>(base[I]) + i, r[I]);
+    if constexpr (((Op::kWrite >> I) & 1u) && std::is_same<T, f16_t>::value) {
+      // the fp16 copy is the rounding of the fp32 value that its master list gets: kept apart from the
+      // arithmetic before it, which the compiler would fold into one conversion of the unrounded sum
+      float v[kVec];
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        v[k] = r[I][k];
+        asm("" : "+v"(v[k]));
+      }
+      MtaIO<T>::store(reinterpret_cast<T*>(base[I]) + i, v);
+    } else if constexpr ((Op::kWrite >> I) & 1u) {
+      MtaIO<T>::store(reinterpret_cast<T*>(base[I]) + i, r[I]);
+    }
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::store_vec(r, base, i);
   }
   static __device__ __forceinline__ void load_one(float (&r)[D][1], void* const (&base)[D], int i) {

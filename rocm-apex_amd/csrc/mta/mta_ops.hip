@@ -391,6 +391,15 @@ void mt_adam_undo(const MtaMeta& m, int g_t, int out_t, int* noop, const AdamArg
 // =============================================================================================
 // SGD with momentum (reference csrc/multi_tensor_sgd_kernel.cu:29-139)
 // =============================================================================================
+// a b + c d with both products rounded.  The scalar tail of SGD has always been computed so (its two
+// products were one packed multiplication); the empty statements keep them from being fused into the sum.
+__device__ __forceinline__ float two_products(float a, float b, float c, float d) {
+  float p = a * b, q = c * d;
+  asm("" : "+v"(p));
+  asm("" : "+v"(q));
+  return p + q;
+}
+
 template <int D>
 struct SgdOp : MtaOpBase {
   static constexpr unsigned kRead = 0b0111, kWrite = (D == 4) ? 0b1110 : 0b0110;
@@ -407,8 +416,9 @@ struct SgdOp : MtaOpBase {
       float mom = r[2][k];
       if (a.wd != 0.f && !a.wd_after_momentum) g += a.wd * w;
       if (a.momentum != 0.f) {
-        if (!a.first_run) mom = mom * a.momentum + (1.f - a.dampening) * g;
-        else mom = g;
+        if (a.first_run) mom = g;
+        else if constexpr (N > 1) mom = mom * a.momentum + (1.f - a.dampening) * g;
+        else mom = two_products(mom, a.momentum, 1.f - a.dampening, g);
         if (a.nesterov) g += a.momentum * mom;
         else g = mom;
       }
