@@ -669,8 +669,11 @@ struct Plan {
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tile width and K splits by a count of K-tile steps of the busiest CU: rounds of workgroups x their K
-// tiles x the tile's width (a 128-wide tile runs at about 0.8 of the wide one's rate: its A fragments feed
-// half the MFMAs), plus the partials' traffic for splits.
+// tiles (and six for fill and epilogue) x the tile's step, plus the partials' traffic for splits.  A step is
+// about 1.5 us for the wide tile and 1.0-1.1 for the 128-wide one, whose A fragments feed half the MFMAs.
+// Either side of the choices, us: 8192 x 1024 x 2736: 128-wide 54, wide 77, wide in two splits 70;
+// 1024 x 2736 x 8192: 128-wide in two splits 69, unsplit 108, wide in four 69; 777 x 5504 x 2048 gated: wide
+// 49, 128-wide 56; 8192 x 2736 x 1024 gradient: 128-wide 87, wide 91.
 inline Plan make_plan(const FfnArgs& g, int cus) {
   const int hn256 = g.op == kFfnGated ? 128 : 256;
   Plan best{256, 1, g.k};
@@ -682,9 +685,9 @@ inline Plan make_plan(const FfnArgs& g, int cus) {
       const int chunk = (int)(cdiv(cdiv(g.k, sp), BK) * BK);
       const int real = (int)cdiv(g.k, chunk);
       if (real != sp) continue;
-      const double steps = (double)cdiv(tiles * sp, cus) * (chunk / BK + 6.0) * (bn == 256 ? 1.0 : 0.62);
-      // a K-tile step of the wide tile is about 0.9 us; partials move 8 bytes an output and split at 4 TB/s
-      const double extra = sp > 1 ? (double)g.m * g.n * sp * 8 / 4e6 / 0.9 + 5.0 : 0.0;
+      const double steps = (double)cdiv(tiles * sp, cus) * (chunk / BK + 6.0) * (bn == 256 ? 1.0 : 0.66);
+      // partials move 8 bytes an output and split at 4 TB/s, the join is a launch
+      const double extra = sp > 1 ? ((double)g.m * g.n * sp * 8 / 4e6 + 5.0) / 1.5 : 0.0;
       if (steps + extra < cost) {
         cost = steps + extra;
         best = Plan{bn, sp, chunk};

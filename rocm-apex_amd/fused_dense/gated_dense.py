@@ -10,6 +10,7 @@ import torch
 from torch import nn
 
 from .. import _native
+from .._autocast_utils import _active_device, _autocast_disabled, _cast_if_autocast_enabled
 from ..amp import half_function
 
 _ACTIVATIONS = ("silu", "gelu")
@@ -72,6 +73,12 @@ def _torch_gated_dense(x, w1, b1, w2, b2, activation):
 
 
 def _gated_dense(input, weight1, bias1, weight2, bias2, activation="silu"):
+    """:func:`fused_dense_gated_dense_function`: ``(input, weight1, bias1, weight2, bias2, activation)``, the
+    biases ``None`` where there are none.  Under autocast the tensors are cast to its dtype."""
+    if _active_device() is not None:
+        args = _cast_if_autocast_enabled(input, weight1, bias1, weight2, bias2)
+        with _autocast_disabled():
+            return _gated_dense(*args, activation)
     _check(input, weight1, bias1, weight2, bias2, activation)
     if not _native_ok(input, weight1, weight2):
         return _torch_gated_dense(input, weight1, bias1, weight2, bias2, activation)

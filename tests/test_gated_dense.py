@@ -100,6 +100,27 @@ def test_cpu_block_and_module():
         assert m(x).shape == (2, 3, 4) and FusedDenseGatedDense(6, 10, 4).bias1 is None
 
 
+def _autocast(dev, dtype):
+    m = FusedDenseGatedDense(16, 24, 8, bias=True).to(dev)
+    x = torch.randn(5, 16, device=dev)
+    with torch.autocast(dev, dtype=dtype):
+        y = m(x)
+    assert y.dtype == dtype
+    y.float().sum().backward()
+    assert all(p.grad.dtype == torch.float32 and p.grad.isfinite().all() for p in m.parameters())
+    low = [p.detach().to(dtype) for p in (m.weight1, m.bias1, m.weight2, m.bias2)]
+    assert torch.equal(y, fused_dense_gated_dense_function(x.to(dtype), *low))
+
+
+def test_cpu_autocast():
+    _autocast("cpu", torch.bfloat16)
+
+
+@pytest.mark.gpu
+def test_gpu_autocast():
+    _autocast("cuda", torch.float16)
+
+
 def _refusals(dev):
     f = fused_dense_gated_dense_function
     z = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device=dev)
