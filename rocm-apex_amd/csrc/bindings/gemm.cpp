@@ -125,8 +125,8 @@ at::Tensor vec16(const at::Tensor& t) {
 }
 
 void ffn_run(int op, const at::Tensor& a, bool a_kmajor, const at::Tensor& b, bool b_kmajor, int64_t m, int64_t n,
-             int64_t k, const at::Tensor& c, int act, const at::Tensor& bias, const at::Tensor& aux_in,
-             const at::Tensor& aux_out) {
+             int64_t k, const at::Tensor& c, int act, const at::Tensor& bias, const at::Tensor& hi,
+             const at::Tensor& lo) {
   TORCH_CHECK(m < (int64_t(1) << 31) && n < (int64_t(1) << 30) && k < (int64_t(1) << 31), "gated_ffn: sizes too large");
   FfnArgs g{};
   g.a = a.data_ptr();
@@ -144,8 +144,8 @@ void ffn_run(int op, const at::Tensor& a, bool a_kmajor, const at::Tensor& b, bo
   g.op = op;
   g.act = act;
   g.bias = bias.defined() ? bias.data_ptr() : nullptr;
-  g.aux_in = aux_in.defined() ? aux_in.data_ptr() : nullptr;
-  g.aux_out = aux_out.defined() ? aux_out.data_ptr() : nullptr;
+  g.au_hi = hi.defined() ? (uint16_t*)hi.data_ptr<int16_t>() : nullptr;
+  g.au_lo = lo.defined() ? lo.data_ptr<uint8_t>() : nullptr;
   TORCH_CHECK(ffn_supported(g), "gated_ffn: unsupported sizes or alignment (fp16 / bf16, widths multiples of 8)");
   const int cus = device_cus(a.get_device());
   at::Tensor ws;
@@ -174,7 +174,7 @@ at::Tensor ffn_bias(const OT& b, int64_t n, const at::Tensor& x) {
   return vec16(*b);
 }
 
-// (y, h, au); h and au (the backward's inputs) are undefined unless save
+// (y, h, au's planes); the last three (the backward's inputs) are undefined unless save
 std::vector<at::Tensor> ffn_forward(const at::Tensor& x_, const at::Tensor& w1_, const OT& b1_, const at::Tensor& w2_,
                                     const OT& b2_, int64_t act, bool save) {
   TORCH_CHECK(x_.is_cuda(), "gated_ffn: GPU tensors expected");
@@ -183,29 +183,34 @@ std::vector<at::Tensor> ffn_forward(const at::Tensor& x_, const at::Tensor& w1_,
   at::Tensor x = vec16(x_), w1 = vec16(w1_), w2 = vec16(w2_);
   const int64_t m = x.size(0), k = x.size(1), f = w2.size(1), n = w2.size(0);
   at::Tensor b1 = ffn_bias(b1_, 2 * f, x), b2 = ffn_bias(b2_, n, x);
-  at::Tensor h = at::empty({m, f}, x.options()), y = at::empty({m, n}, x.options()), au;
-  if (save) au = at::empty({m, 2 * f}, x.options());
+  at::Tensor h = at::empty({m, f}, x.options()), y = at::empty({m, n}, x.options()), hi, lo;
+  if (save) {
+    hi = at::empty({m, 2 * f}, x.options().dtype(at::kShort));
+    lo = at::empty({m, 2 * f}, x.options().dtype(at::kByte));
+  }
   if (m > 0) {
-    ffn_run(kFfnGated, x, true, w1, true, m, f, k, h, (int)act, b1, at::Tensor(), au);
+    ffn_run(kFfnGated, x, true, w1, true, m, f, k, h, (int)act, b1, hi, lo);
     ffn_run(kFfnPlain, h, true, w2, true, m, n, f, y, 0, b2, at::Tensor(), at::Tensor());
   }
-  return {y, save ? h : at::Tensor(), au};
+  return {y, save ? h : at::Tensor(), hi, lo};
 }
 
 // (dx, dw1, db1, dw2, db2), undefined where not needed
 std::vector<at::Tensor> ffn_backward(const at::Tensor& dy_, const at::Tensor& x_, const at::Tensor& w1_,
-                                     const at::Tensor& w2_, const at::Tensor& h, const at::Tensor& au, int64_t act,
-                                     bool need_dx, bool need_dw1, bool need_db1, bool need_dw2, bool need_db2) {
+                                     const at::Tensor& w2_, const at::Tensor& h, const at::Tensor& hi,
+                                     const at::Tensor& lo, int64_t act, bool need_dx, bool need_dw1, bool need_db1, bool need_dw2, bool need_db2) {
   TORCH_CHECK(x_.is_cuda(), "gated_ffn: GPU tensors expected");
   const c10::hip::HIPGuard guard(x_.get_device());
   ffn_check(x_, w1_, w2_, act);
   at::Tensor dy = vec16(dy_), x = vec16(x_), w1 = vec16(w1_), w2 = vec16(w2_);
   const int64_t m = x.size(0), k = x.size(1), f = w2.size(1), n = w2.size(0);
-  auto is = [&](const at::Tensor& t, int64_t c) {
-    return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == x.scalar_type() && t.dim() == 2 &&
+  auto is = [&](const at::Tensor& t, int64_t c, at::ScalarType type) {
+    return t.is_cuda() && t.get_device() == x.get_device() && t.scalar_type() == type && t.dim() == 2 &&
            t.size(0) == m && t.size(1) == c && t.is_contiguous();
   };
-  TORCH_CHECK(is(dy, n) && is(h, f) && is(au, 2 * f), "gated_ffn: backward operands do not fit");
+  TORCH_CHECK(is(dy, n, x.scalar_type()) && is(h, f, x.scalar_type()) && is(hi, 2 * f, at::kShort) &&
+                  is(lo, 2 * f, at::kByte),
+              "gated_ffn: backward operands do not fit");
   const at::Tensor none;
   at::Tensor dx, dw1, db1, dw2, db2;
   if (m == 0) {
@@ -223,7 +228,7 @@ std::vector<at::Tensor> ffn_backward(const at::Tensor& dy_, const at::Tensor& x_
   if (need_db2) db2 = colsum(dy, x.scalar_type());
   if (need_dx || need_dw1 || need_db1) {
     at::Tensor dau = at::empty({m, 2 * f}, x.options());
-    ffn_run(kFfnDGated, dy, true, w2, false, m, f, n, dau, (int)act, none, au, none);
+    ffn_run(kFfnDGated, dy, true, w2, false, m, f, n, dau, (int)act, none, hi, lo);
     if (need_dw1) {
       dw1 = at::empty({2 * f, k}, x.options());
       ffn_run(kFfnPlain, dau, false, x, false, 2 * f, k, m, dw1, 0, none, none, none);

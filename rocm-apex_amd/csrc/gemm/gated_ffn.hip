@@ -49,8 +49,8 @@ struct Params {
   int64_t lda, ldb, ldc;
   int M, N, K;
   const void* bias;
-  const void* aux_in;
-  void* aux_out;
+  uint16_t* au_hi;  // [M][2N] pre-activations a | u (gated: written unless null; dgated: read)
+  uint8_t* au_lo;
   float* part;  // split-K partials [splits][M][N], or null
   int kchunk;
 };
@@ -186,6 +186,42 @@ __device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
                     (uint32_t)from_f<T>(v[2]).x | (uint32_t)from_f<T>(v[3]).x << 16);
 }
 
+// Pre-activations are kept for the backward as the upper 24 bits of their fp32 value (15 bits of
+// mantissa) in a 16- and an 8-bit plane: rounded to bf16 / fp16 they would put two more roundings of the type
+// into dx and dW1 (0.0030 instead of 0.0024 of their norm for bf16, where the result's own rounding is
+// 0.0017), for 1 % of the time.  The low bits are cut off: a NaN stays one, nothing overflows.
+__device__ __forceinline__ uint2 hi4(const float (&v)[4]) {
+  return make_uint2(__builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u),
+                    __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u));
+}
+__device__ __forceinline__ uint32_t lo4(const float (&v)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501u);
+  const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x0c0c0501u);
+  return a | b << 16;
+}
+__device__ __forceinline__ void join8(float (&v)[8], uint4 hi, uint2 lo) {
+  const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[2] = {lo.x, lo.y};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t h16 = e & 1 ? h[e >> 1] & 0xffff0000u : h[e >> 1] << 16;
+    v[e] = __uint_as_float(h16 | ((l[e >> 2] >> (8 * (e & 3))) & 0xffu) << 8);
+  }
+}
+
+// 8-byte stores of a [256][W] 8-bit LDS image
+template <int W, int PITCH>
+__device__ __forceinline__ void store_bytes(const uint8_t* img, uint8_t* C, int64_t ldc, int row0, int col0, int M, int N,
+                                            int tid) {
+  constexpr int V = W / 8;
+  const int ch = tid % V, gc = col0 + 8 * ch;
+  if (gc >= N) return;
+#pragma unroll 4
+  for (int r = tid / V; r < BM; r += NT / V) {
+    if (row0 + r >= M) break;
+    *reinterpret_cast<uint2*>(C + (int64_t)(row0 + r) * ldc + gc) = *reinterpret_cast<const uint2*>(img + r * PITCH + 8 * ch);
+  }
+}
+
 // 16-byte stores of a [256][W] 16-bit LDS image to rows row0.., columns col0.. of C
 template <typename T, int W, int PITCH>
 __device__ __forceinline__ void store_image(const uint16_t* img, T* C, int64_t ldc, int row0, int col0, int M, int N,
@@ -263,7 +299,11 @@ template <> struct Ring<128> {
 template <int BN, int OP>
 constexpr size_t lds_bytes() {
   const size_t ops = Ring<BN>::kBytes;
-  const size_t epi = OP == kFfnDGated ? (size_t)128 * (BN + 4) * 4 : (size_t)BM * (BN + 8) * 2;
+  // gated: h beside the lower plane, or the upper plane alone
+  const size_t epi = OP == kFfnDGated ? (size_t)128 * (BN + 4) * 4
+                     : OP == kFfnGated ? (size_t)BM * (BN / 2 + 8) * 2 + (size_t)BM * (BN + 8)
+                                       : (size_t)BM * (BN + 8) * 2;
+  static_assert(Ring<256>::kBytes >= 256 * 264 * 2, "the upper plane's image");
   return ops > epi ? ops : epi;
 }
 
@@ -402,9 +442,10 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
     __syncthreads();
     store_image<T, BN, PITCH>(lds, (T*)P.C, P.ldc, row0, col0, P.M, P.N, tid);
   } else if constexpr (OP == kFfnGated) {
-    // add the biases; the pre-activations (rounded to the 16-bit type: what the backward recomputes the
-    // activation from) leave through one image [a | u], h through a second
+    // biases; then the upper plane of the pre-activations leaves through one image [a | u], and their
+    // lower plane with h through a second
     constexpr int PITCH = BN + 8, HP = HN + 8, NH = NJ / 2;
+    uint8_t* low = reinterpret_cast<uint8_t*>(lds + BM * HP);
 #pragma unroll
     for (int j = 0; j < NH; ++j)
 #pragma unroll
@@ -420,25 +461,20 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
           float a[4], u[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            a[e] = acc[i][j][4 * q + e] + ba[e];
-            u[e] = acc[i][j + NH][4 * q + e] + bu[e];
+            a[e] = acc[i][j][4 * q + e] += ba[e];
+            u[e] = acc[i][j + NH][4 * q + e] += bu[e];
           }
-          if (P.aux_out != nullptr) {
+          if (P.au_hi != nullptr) {
             uint16_t* at = lds + (wm * 128 + 32 * i + lrow) * PITCH + lc;
-            *reinterpret_cast<uint2*>(at) = pack4<T>(a);
-            *reinterpret_cast<uint2*>(at + HN) = pack4<T>(u);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float d;
-            acc[i][j][4 * q + e] = activate<ACT>(a[e], d) * u[e];
+            *reinterpret_cast<uint2*>(at) = hi4(a);
+            *reinterpret_cast<uint2*>(at + HN) = hi4(u);
           }
         }
       }
-    if (P.aux_out != nullptr) {
+    if (P.au_hi != nullptr) {
       __syncthreads();
-      store_image<T, HN, PITCH>(lds, (T*)P.aux_out, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
-      store_image<T, HN, PITCH>(lds + HN, (T*)P.aux_out + P.N, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
+      store_image<bf16_t, HN, PITCH>(lds, (bf16_t*)P.au_hi, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
+      store_image<bf16_t, HN, PITCH>(lds + HN, (bf16_t*)P.au_hi + P.N, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
       __syncthreads();
     }
 #pragma unroll
@@ -447,30 +483,48 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
       for (int q = 0; q < 4; ++q)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          *reinterpret_cast<uint2*>(lds + (wm * 128 + 32 * i + lrow) * HP + wn * (HN / 2) + 32 * j + 8 * q + lcol) =
-              pack4<T>(v);
+          const int r = wm * 128 + 32 * i + lrow, lc = wn * (HN / 2) + 32 * j + 8 * q + lcol;
+          float a[4], u[4], h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float d;
+            a[e] = acc[i][j][4 * q + e];
+            u[e] = acc[i][j + NH][4 * q + e];
+            h[e] = activate<ACT>(a[e], d) * u[e];
+          }
+          if (P.au_hi != nullptr) {
+            *reinterpret_cast<uint32_t*>(low + r * PITCH + lc) = lo4(a);
+            *reinterpret_cast<uint32_t*>(low + r * PITCH + HN + lc) = lo4(u);
+          }
+          *reinterpret_cast<uint2*>(lds + r * HP + lc) = pack4<T>(h);
         }
     __syncthreads();
     store_image<T, HN, HP>(lds, (T*)P.C, P.ldc, row0, col0, P.M, P.N, tid);
+    if (P.au_hi != nullptr) {
+      store_bytes<HN, PITCH>(low, P.au_lo, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
+      store_bytes<HN, PITCH>(low + HN, P.au_lo + P.N, 2 * (int64_t)P.N, row0, col0, P.M, P.N, tid);
+    }
   } else {
     // dh stays fp32: 128 rows at a time through LDS, then 8 consecutive columns a thread with a and u.  These
-    // are fetched for all of a thread's rows of a half at once, the second half's into the registers
-    // that the first half's free (row by row, four at a time, their latency was a third of the kernel at
-    // 1024-deep products).
-    constexpr int CST = BN + 4, V = BN / 8, RPP = NT / V, IT = 128 / RPP;
+    // are fetched AH rows ahead, the first of them before the staging (row by row, four at a time, their
+    // latency was a third of the kernel at 1024-deep products).
+    constexpr int CST = BN + 4, V = BN / 8, RPP = NT / V, IT = 128 / RPP, AH = 8;
+    static_assert(IT % AH == 0, "the fetch ring's slots follow the row index");
     float* cs = reinterpret_cast<float*>(lds);
     const int ch = tid % V, gc = col0 + 8 * ch;
-    const T* au = (const T*)P.aux_in + min(gc, P.N - 8);  // clamped: loads past the edges are not used
+    const int64_t gcc = min(gc, P.N - 8);  // clamped: loads past the edges are not used
     T* out = (T*)P.C;
-    uint4 pa[IT], pu[IT];
-    auto fetch = [&](int half, int it) {
-      const int64_t at = (int64_t)min(row0 + 128 * half + tid / V + RPP * it, P.M - 1) * P.ldc;
-      pa[it] = *reinterpret_cast<const uint4*>(au + at);
-      pu[it] = *reinterpret_cast<const uint4*>(au + at + P.N);
+    uint4 pa[AH], pu[AH];
+    uint2 la[AH], lu[AH];
+    auto fetch = [&](int n) {  // row n of the thread's 2 IT
+      const int64_t at = (int64_t)min(row0 + tid / V + RPP * n, P.M - 1) * P.ldc + gcc;
+      pa[n % AH] = *reinterpret_cast<const uint4*>(P.au_hi + at);
+      pu[n % AH] = *reinterpret_cast<const uint4*>(P.au_hi + at + P.N);
+      la[n % AH] = *reinterpret_cast<const uint2*>(P.au_lo + at);
+      lu[n % AH] = *reinterpret_cast<const uint2*>(P.au_lo + at + P.N);
     };
 #pragma unroll
-    for (int it = 0; it < IT; ++it) fetch(0, it);
+    for (int n = 0; n < AH; ++n) fetch(n);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       if (wm == half) {
@@ -486,11 +540,11 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
       __syncthreads();
 #pragma unroll
       for (int it = 0; it < IT; ++it) {
-        const int r = tid / V + RPP * it, gr = row0 + 128 * half + r;
+        const int r = tid / V + RPP * it, gr = row0 + 128 * half + r, n = half * IT + it;
         float a[8], u[8], g[8], da[8], du[8];
-        Vec8<T>::load(a, reinterpret_cast<const T*>(&pa[it]));
-        Vec8<T>::load(u, reinterpret_cast<const T*>(&pu[it]));
-        if (half == 0) fetch(1, it);
+        join8(a, pa[n % AH], la[n % AH]);
+        join8(u, pu[n % AH], lu[n % AH]);
+        if (n + AH < 2 * IT) fetch(n + AH);
         Vec8<float>::load(g, cs + r * CST + 8 * ch);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -604,10 +658,13 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
       v[g] = s + (P.bias != nullptr ? to_f(((const T*)P.bias)[(int64_t)g * P.N + gc]) : 0.f);
     }
     if constexpr (GATED) {
-      if (P.aux_out != nullptr) {
-        T* au = (T*)P.aux_out + (int64_t)tok * 2 * P.N + gc;
-        au[0] = from_f<T>(v[0]);
-        au[P.N] = from_f<T>(v[1]);
+      if (P.au_hi != nullptr) {
+        const int64_t at = (int64_t)tok * 2 * P.N + gc;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          P.au_hi[at + g * P.N] = (uint16_t)(__float_as_uint(v[g]) >> 16);
+          P.au_lo[at + g * P.N] = (uint8_t)(__float_as_uint(v[g]) >> 8);
+        }
       }
       float d;
       v[0] = activate<ACT>(v[0], d) * v[1];
@@ -618,8 +675,8 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
 
 template <typename T, bool GATED, int ACT, int TM, int NW>
 void launch_few(const FfnArgs& g, hipStream_t s) {
-  Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.aux_in,
-           g.aux_out, nullptr, g.k};
+  Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.au_hi,
+           g.au_lo, nullptr, g.k};
   const size_t lds = (size_t)NW * TM * 16 * (16 * (GATED ? 2 : 1) + 4) * sizeof(float);
   hipLaunchKernelGGL((ffn_few_kernel<T, GATED, ACT, TM, NW>), dim3((unsigned)((g.n + 15) / 16)), dim3(NW * 64), lds, s, P);
 }
@@ -700,8 +757,8 @@ inline Plan make_plan(const FfnArgs& g, int cus) {
 template <typename T, bool AK, bool BKM, int OP, int BN, int ACT>
 void launch(const FfnArgs& g, const Plan& p, int cus, hipStream_t s) {
   constexpr int HN = OP == kFfnGated ? BN / 2 : BN;
-  Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.aux_in,
-           g.aux_out, p.splits > 1 ? g.ws : nullptr, p.kchunk};
+  Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.au_hi,
+           g.au_lo, p.splits > 1 ? g.ws : nullptr, p.kchunk};
   const unsigned tiles = (unsigned)(cdiv(g.m, BM) * cdiv(g.n, HN));
   hipLaunchKernelGGL((ffn_gemm_kernel<T, AK, BKM, OP, BN, ACT>), dim3(tiles, p.splits), dim3(NT),
                      (lds_bytes<BN, OP>()), s, P);
@@ -725,7 +782,8 @@ bool ffn_supported(const FfnArgs& g) {
   if (g.dtype != kF16 && g.dtype != kBF16) return false;
   if (g.m <= 0 || g.n <= 0 || g.k <= 0) return false;
   auto al = [](const void* p) { return ((uintptr_t)p & 15u) == 0; };
-  if (!al(g.a) || !al(g.b) || !al(g.c) || !al(g.bias) || !al(g.aux_in) || !al(g.aux_out)) return false;
+  if (!al(g.a) || !al(g.b) || !al(g.c) || !al(g.bias) || !al(g.au_hi) || !al(g.au_lo)) return false;
+  if ((g.au_hi == nullptr) != (g.au_lo == nullptr)) return false;
   if (g.n % 8 || g.lda % 8 || g.ldb % 8 || g.ldc % 8) return false;
   if ((g.a_kmajor || g.b_kmajor) && g.k % 8) return false;
   if (!g.a_kmajor && g.m % 8) return false;
@@ -735,7 +793,7 @@ bool ffn_supported(const FfnArgs& g) {
   switch (g.op) {
     case kFfnPlain: return !(!g.a_kmajor && g.b_kmajor);
     case kFfnGated: return g.a_kmajor && g.b_kmajor;
-    case kFfnDGated: return g.a_kmajor && !g.b_kmajor && g.aux_in != nullptr && g.ldc == 2 * (int64_t)g.n;
+    case kFfnDGated: return g.a_kmajor && !g.b_kmajor && g.au_hi != nullptr && g.ldc == 2 * (int64_t)g.n;
     default: return false;
   }
 }

@@ -49,19 +49,19 @@ class FusedDenseGatedDenseFunc(torch.autograd.Function):
         ext = _ext()
         x = input.reshape(-1, input.size(-1))
         ctx.act = ext.ACT_SILU if activation == "silu" else ext.ACT_GELU
-        y, h, au = ext.forward(x, weight1, bias1, weight2, bias2, ctx.act, save)
+        y, h, hi, lo = ext.forward(x, weight1, bias1, weight2, bias2, ctx.act, save)
         if save:
-            ctx.save_for_backward(x, weight1, weight2, h, au)
+            ctx.save_for_backward(x, weight1, weight2, h, hi, lo)  # hi, lo: the pre-activations' two planes
         ctx.shape = input.shape
         return y.view(input.shape[:-1] + (weight2.size(0),))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        x, weight1, weight2, h, au = ctx.saved_tensors
+        x, weight1, weight2, h, hi, lo = ctx.saved_tensors
         need = ctx.needs_input_grad
         dx, dw1, db1, dw2, db2 = _ext().backward(grad_output.reshape(-1, grad_output.size(-1)), x, weight1, weight2,
-                                                 h, au, ctx.act, need[0], need[1], need[2], need[3], need[4])
+                                                 h, hi, lo, ctx.act, need[0], need[1], need[2], need[3], need[4])
         return (dx.view(ctx.shape) if dx is not None else None), dw1, db1, dw2, db2, None, None
 
 
