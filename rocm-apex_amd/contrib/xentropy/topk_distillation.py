@@ -83,28 +83,29 @@ def _torch_backward(grad_loss, logits, teacher_logits, teacher_indices, temperat
     return torch.where((some | bad)[:, None], dx, torch.zeros_like(dx)).to(logits.dtype)
 
 
-class SoftmaxTopKDistillationLoss(torch.autograd.Function):
+class _TorchTopKDistillation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher_logits, teacher_indices, temperature=1.0, half_to_float=False):
-        temperature = float(temperature)
-        _check(logits, teacher_logits, teacher_indices, temperature)
-        if ctx.needs_input_grad[1]:
-            raise ValueError("the teacher takes no gradient: detach its logits")
-        if _native.use_native(logits):
-            losses, stats = _ext().topk_distill_forward(logits, teacher_logits, teacher_indices, temperature)
-        else:
-            losses, stats = _torch_forward(logits, teacher_logits, teacher_indices, temperature), None
-        ctx.save_for_backward(logits, teacher_logits, teacher_indices, stats)
+    def forward(ctx, logits, teacher_logits, teacher_indices, temperature, half_to_float):
+        ctx.save_for_backward(logits, teacher_logits, teacher_indices)
         ctx.temperature = temperature
+        losses = _torch_forward(logits, teacher_logits, teacher_indices, temperature)
         return losses if half_to_float else losses.to(logits.dtype)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, teacher_logits, teacher_indices, stats = ctx.saved_tensors
-        if stats is not None:
-            grad = _ext().topk_distill_backward(grad_loss, logits, stats, teacher_logits, teacher_indices,
-                                                ctx.temperature)
-        else:
-            grad = _torch_backward(grad_loss, logits, teacher_logits, teacher_indices, ctx.temperature)
-        return grad, None, None, None, None
+        return _torch_backward(grad_loss, *ctx.saved_tensors, ctx.temperature), None, None, None, None
+
+
+class SoftmaxTopKDistillationLoss:
+    """See the module's documentation; used through :meth:`apply` like the other losses here."""
+
+    @staticmethod
+    def apply(logits, teacher_logits, teacher_indices, temperature=1.0, half_to_float=False):
+        temperature = float(temperature)
+        _check(logits, teacher_logits, teacher_indices, temperature)
+        if teacher_logits.requires_grad and torch.is_grad_enabled():
+            raise ValueError("the teacher takes no gradient: detach its logits")
+        if _native.use_native(logits):
+            return _ext().topk_distill(logits, teacher_logits, teacher_indices, temperature, bool(half_to_float))
+        return _TorchTopKDistillation.apply(logits, teacher_logits, teacher_indices, temperature, bool(half_to_float))

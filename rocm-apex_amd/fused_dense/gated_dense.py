@@ -43,28 +43,6 @@ def _native_ok(x, w1, w2):
             and w2.size(0) % 8 == 0 and w2.size(1) % 8 == 0 and x.size(-1) > 0 and w2.size(0) > 0)
 
 
-class FusedDenseGatedDenseFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, input, weight1, bias1, weight2, bias2, activation, save):
-        ext = _ext()
-        x = input.reshape(-1, input.size(-1))
-        ctx.act = ext.ACT_SILU if activation == "silu" else ext.ACT_GELU
-        y, h, hi, lo = ext.forward(x, weight1, bias1, weight2, bias2, ctx.act, save)
-        if save:
-            ctx.save_for_backward(x, weight1, weight2, h, hi, lo)  # hi, lo: the pre-activations' two planes
-        ctx.shape = input.shape
-        return y.view(input.shape[:-1] + (weight2.size(0),))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_output):
-        x, weight1, weight2, h, hi, lo = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw1, db1, dw2, db2 = _ext().backward(grad_output.reshape(-1, grad_output.size(-1)), x, weight1, weight2,
-                                                 h, hi, lo, ctx.act, need[0], need[1], need[2], need[3], need[4])
-        return (dx.view(ctx.shape) if dx is not None else None), dw1, db1, dw2, db2, None, None
-
-
 def _torch_gated_dense(x, w1, b1, w2, b2, activation):
     au = torch.nn.functional.linear(x, w1, b1)
     a, u = au.chunk(2, dim=-1)
@@ -82,9 +60,10 @@ def _gated_dense(input, weight1, bias1, weight2, bias2, activation="silu"):
     _check(input, weight1, bias1, weight2, bias2, activation)
     if not _native_ok(input, weight1, weight2):
         return _torch_gated_dense(input, weight1, bias1, weight2, bias2, activation)
-    save = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (input, weight1, bias1, weight2, bias2))
-    return FusedDenseGatedDenseFunc.apply(input, weight1, bias1, weight2, bias2, activation, save)
+    ext = _ext()
+    y = ext.gated_ffn(input.reshape(-1, input.size(-1)), weight1, bias1, weight2, bias2,
+                      ext.ACT_SILU if activation == "silu" else ext.ACT_GELU)
+    return y if input.dim() == 2 else y.view(input.shape[:-1] + (weight2.size(0),))
 
 
 fused_dense_gated_dense_function = half_function(_gated_dense)

@@ -53,26 +53,6 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
-class _FusedQKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        ext = _native.require("fused_transformer").fused_transformer
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.meta = (eps, interleaved)
-        return tuple(ext.qk_norm_rope_forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        ext = _native.require("fused_transformer").fused_transformer
-        dq, dk, dqw, dkw = ext.qk_norm_rope_backward(_rows(gq), _rows(gk), q, k, q_weight, k_weight, cos, sin,
-                                                     positions, *ctx.meta)
-        if dqw is not None:
-            dqw, dkw = dqw.view_as(q_weight), dkw.view_as(k_weight)
-        return dq, dk, dqw, dkw, None, None, None, None, None
-
-
 def fused_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, interleaved=False):
     """Normed and rotated ``(q', k')`` of queries ``[..., heads, d]`` and keys ``[..., kv_heads, d]``
     (one or two leading token axes, the same for both; any strides with d contiguous, e.g. views of a
@@ -122,6 +102,7 @@ def fused_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, 
     flat = q.dim() == 3
     if flat:
         q, k, positions = q.unsqueeze(0), k.unsqueeze(0), positions.unsqueeze(0)
-    qo, ko = _FusedQKNormRope.apply(_rows(q), _rows(k), q_weight, k_weight, cos, sin, positions, float(eps),
-                                    bool(interleaved))
+    ext = _native.require("fused_transformer").fused_transformer
+    qo, ko = ext.qk_norm_rope(_rows(q), _rows(k), q_weight, k_weight, cos, sin, positions, float(eps),
+                              bool(interleaved))
     return (qo[0], ko[0]) if flat else (qo, ko)

@@ -266,3 +266,11 @@ def test_gpu_other_stream_captured_graph_and_repeatability(m):
         got = [o.clone() for o in outs]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_gpu_no_second_derivative():
+    x, w1, b1, w2, b2, dy = _inputs("cuda", 5, 64, 72, 40, torch.bfloat16, False)
+    y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, x, dy, create_graph=True)

@@ -253,3 +253,11 @@ def test_gpu_other_stream_and_captured_graph():
         got = [o.clone() for o in outs]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_gpu_no_second_derivative():
+    q, k, qw, kw, cos, sin, pos, gq, _ = _case("cuda", (4,), 2, 1, 32, 16, False, torch.float32, torch.float32, False)
+    qo, _ = fused_qk_norm_rope(q, k, qw, kw, cos, sin, pos)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(qo, q, gq, create_graph=True)

@@ -247,3 +247,10 @@ def test_gpu_other_stream_captured_graph_and_repeatability():
         got = [o.clone() for o in outs]
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_gpu_no_second_derivative():
+    x, z, idx, w = _case("cuda", 5, 99, 4, torch.float32)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(SoftmaxTopKDistillationLoss.apply(x, z, idx, 1.0, True), x, w, create_graph=True)
