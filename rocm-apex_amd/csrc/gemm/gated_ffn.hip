@@ -566,9 +566,10 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 // ---------------------------------------------------------------------------------------------
 // Few rows (a token each of up to 32 sequences): the weights are read once and nothing else counts.
 // A workgroup owns 16 outputs (16 rows of Wg and of Wu, or of W2) and its NW waves split K; the weights
-// go straight from memory to the MFMA operand (16 rows x 32 k a load), U steps in flight per wave, x comes
-// from the caches.  The waves' partial tiles meet in LDS in a fixed order, where the block's
-// epilogue (bias, activation, product) runs in fp32.
+// go straight from memory to the MFMA operand (16 rows x 32 k a load), U steps in flight per wave.  x goes
+// through LDS by DMA, whole 64 U byte runs of a row at a time: read like the weights, 64 bytes of 16 rows a
+// load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels instead of 24).  The waves' partial tiles
+// meet in LDS in a fixed order, where the block's epilogue (bias, activation, product) runs in fp32.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -586,12 +587,19 @@ __device__ __forceinline__ f32x4 mma16<f16_t>(i32x4 a, i32x4 b, f32x4 c) {
 
 constexpr int kFewRows = 32;
 
+// floats of LDS: the waves' x tiles, then their partial tiles [NW][16 TM][16 or 32 outputs + 4]
+template <bool GATED, int TM, int NW>
+constexpr int few_lds() {
+  return NW * (TM * 16 * (16 * (GATED ? 2 : 1) + 4) > 1024 ? TM * 16 * (16 * (GATED ? 2 : 1) + 4) : 1024);
+}
+
 template <typename T, bool GATED, int ACT, int TM, int NW>
 __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
-  constexpr int G = GATED ? 2 : 1, U = TM == 1 && !GATED ? 8 : 4;
+  constexpr int G = GATED ? 2 : 1, U = 4 / TM;  // 4 KB of x a wave and group of U steps
+  constexpr int LPR = 4 * U, RPI = 64 / LPR;    // lanes (16-byte chunks) a row of x, rows a DMA instruction
   constexpr int TP = 16 * G + 4;  // floats a token takes in a wave's partial tile
-  extern __shared__ __attribute__((aligned(16))) float part[];  // [NW][16 TM][TP]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  extern __shared__ __attribute__((aligned(16))) float part[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col0 = blockIdx.x * 16, l16 = lane & 15, g8 = 8 * (lane >> 4);
   const int chunk = ((P.K + NW - 1) / NW + 31) / 32 * 32;
   const int k1 = min(P.K, (wave + 1) * chunk);
@@ -604,11 +612,13 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
   for (int g = 0; g < G; ++g)
     rw[g] = __builtin_amdgcn_make_buffer_rsrc((void*)(P.B + ((int64_t)g * P.N + col0) * P.ldb), 0,
                                               (int)(((rows - 1) * P.ldb + P.K) * 2), 0x00027000);
-  const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)P.A, 0, (int)(((P.M - 1) * P.lda + P.K) * 2), 0x00027000);
   const int ow = (int)((l16 * P.ldb + g8) * 2);
-  int ox[TM];
-#pragma unroll
-  for (int t = 0; t < TM; ++t) ox[t] = (int)(((16 * t + l16) * P.lda + g8) * 2);
+  // x tile image [16 TM][32 U]: chunk c of row r at c ^ swz(r), so that a fragment's 16 rows hit all banks
+  const auto swz = [](int r) { return U == 4 ? r & 15 : (r >> 1) & 7; };
+  const i32x4 rx = rsrc(P.A, (P.M - 1) * P.lda + P.K);
+  const uint16_t* xt = reinterpret_cast<const uint16_t*>(part) + wave * 2048;
+  const uint32_t xdst = lds_addr(xt);
+  const int xr = lane / LPR;
   f32x4 acc[G][TM];
 #pragma unroll
   for (int g = 0; g < G; ++g)
@@ -617,28 +627,36 @@ __global__ void __launch_bounds__(NW * 64) ffn_few_kernel(const Params P) {
 
   // U steps of loads, all in flight, then their MFMAs; the last group's loads past the wave's chunk are zeros
   auto group = [&](auto last) {
-    i32x4 wv[U][G], xv[U][TM];
+    i32x4 wv[U][G];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = RPI * i + xr, kc = k + 8 * ((lane % LPR) ^ swz(r));
+      dma(rx, !decltype(last)::value || kc < k1 ? (int)((r * P.lda + kc) * 2) : kOut, xdst + 1024 * i);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const bool in = !decltype(last)::value || k + 32 * u + g8 < k1;
-      const int at = 2 * (k + 32 * u);
 #pragma unroll
       for (int g = 0; g < G; ++g)
-        wv[u][g] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[g], in ? ow + at : kOut, 0, 0));
-#pragma unroll
-      for (int t = 0; t < TM; ++t)
-        xv[u][t] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rx, in ? ox[t] + at : kOut, 0, 0));
+        wv[u][g] = __builtin_bit_cast(
+            i32x4, __builtin_amdgcn_raw_buffer_load_b128(rw[g], in ? ow + 2 * (k + 32 * u) : kOut, 0, 0));
     }
-    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int g = 0; g < G; ++g)
+      for (int t = 0; t < TM; ++t) {
+        const int r = 16 * t + l16, c = 4 * u + (lane >> 4);
+        const i32x4 xv = *reinterpret_cast<const i32x4*>(xt + r * 32 * U + 8 * (c ^ swz(r)));
 #pragma unroll
-        for (int t = 0; t < TM; ++t) acc[g][t] = mma16<T>(wv[u][g], xv[u][t], acc[g][t]);
+        for (int g = 0; g < G; ++g) acc[g][t] = mma16<T>(wv[u][g], xv, acc[g][t]);
+      }
+    // the next group's DMA overwrites the tile
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
   for (; k + 32 * U <= k1; k += 32 * U) group(std::false_type{});
   if (k < k1) group(std::true_type{});
+  __syncthreads();
   // lane: token 16 t + (lane & 15), outputs 4 (lane >> 4) + 0..3
 #pragma unroll
   for (int t = 0; t < TM; ++t)
@@ -677,7 +695,7 @@ template <typename T, bool GATED, int ACT, int TM, int NW>
 void launch_few(const FfnArgs& g, hipStream_t s) {
   Params P{(const uint16_t*)g.a, (const uint16_t*)g.b, g.c, g.lda, g.ldb, g.ldc, g.m, g.n, g.k, g.bias, g.au_hi,
            g.au_lo, nullptr, g.k};
-  const size_t lds = (size_t)NW * TM * 16 * (16 * (GATED ? 2 : 1) + 4) * sizeof(float);
+  const size_t lds = (size_t)few_lds<GATED, TM, NW>() * sizeof(float);
   hipLaunchKernelGGL((ffn_few_kernel<T, GATED, ACT, TM, NW>), dim3((unsigned)((g.n + 15) / 16)), dim3(NW * 64), lds, s, P);
 }
 
