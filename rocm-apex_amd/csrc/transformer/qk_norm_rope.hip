@@ -7,13 +7,17 @@
 // Everything between the one load and the one store of an element is fp32 in registers: the normed
 // value is never rounded to the 16-bit type before it is rotated.
 //
-// Layout: a head of d elements belongs to a group of G lanes (a power of two); each lane holds PV
-// pairs, as two PV-element vectors, so a rotation never leaves the lane and the mean is log2(G)
-// shuffles.  Half-split pairs load the vectors i and i + rot/2, interleaved ones 2 PV consecutive
-// elements.  A group takes HB heads of its token (cosines and sines are loaded once for them, all
-// HB loads are in flight together); neighbouring groups take neighbouring heads, so one load
-// instruction of a wave covers whole cache lines.  Blocks are dealt to q and k in proportion to
-// their heads, so a lane's norm weights and dw sums belong to one tensor for the whole kernel.
+// Layout: a head of d elements belongs to a group of G lanes (one per PV pairs; a wave holds 64 / G
+// groups); each lane holds PV pairs, as two PV-element vectors, so a rotation never leaves the lane and the
+// mean is one sum over the group's lanes.  Half-split pairs load the vectors i and i + rot/2, interleaved ones
+// 2 PV consecutive elements.  Where the rotated part or the rest is no multiple of PV pairs, its last lane
+// starts earlier: the pairs it shares with its neighbour are computed (and stored) twice and counted
+// once, which keeps every access a vector (head 80 with 34 rotated, 32768 x 16 heads bf16: XX us forward and YY
+// backward; one pair a lane and step took 103 and 215).
+// A group takes HB heads of its token (cosines and sines are loaded once for them, all HB loads are in flight
+// together); neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole
+// cache lines.  Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums
+// belong to one tensor for the whole kernel.
 // dw: fp32 per lane over the persistent loop, per block through LDS, then a fixed-order column sum
 // over the blocks (no atomics: the same inputs give the same bits).
 // Positions outside the table give NaN rows (the table is never read past its end).
@@ -43,18 +47,38 @@ __device__ __forceinline__ void store(T* p, const float (&r)[PV]) {
   *reinterpret_cast<Pack<T, PV>*>(p) = v;
 }
 
-// offsets of chunk c's two vectors within the head, and its first pair's index among the rotated
+// A lane's PV pairs.  o1, o2: its two vectors in the head; p0: its first pair's index among the rotated (>=
+// rot/2 for pairs that are not); skip: leading pairs that the lane before it counts.
+struct Chunk { int o1, o2, p0, skip; };
+
+template <int PV> __host__ __device__ inline int cdiv_pv(int n) { return (n + PV - 1) / PV; }
+
 template <int PV, bool INTER>
-__device__ __forceinline__ void chunk_offsets(int c, int d, int rot, int& o1, int& o2) {
+__device__ __forceinline__ Chunk chunk_of(int c, int d, int rot) {
+  const int half = rot >> 1, rest = (d - rot) >> 1;
   if constexpr (INTER) {
-    o1 = 2 * PV * c;
-    o2 = o1 + PV;
+    const int p = min(PV * c, (d >> 1) - PV);
+    return {2 * p, 2 * p + PV, p, PV * c - p};
   } else {
-    const int half = rot >> 1, p = PV * c;
-    const bool in = p < half;
-    o1 = in ? p : rot + (p - half);
-    o2 = o1 + (in ? half : (d - rot) >> 1);
+    const int c1 = cdiv_pv<PV>(half);
+    if (c < c1) {
+      const int p = min(PV * c, half - PV);
+      return {p, half + p, p, PV * c - p};
+    }
+    const int p = min(PV * (c - c1), rest - PV);
+    return {rot + p, rot + rest + p, half, PV * (c - c1) - p};
   }
+}
+
+// sum over a group's G lanes, the same bits in each of them
+__device__ __forceinline__ float group_sum(float v, int G, bool pow2, int first) {
+  if (pow2) {
+    for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+  }
+  float t = 0.f;
+  for (int i = 0; i < G; ++i) t += __shfl(v, first + i, 64);
+  return t;
 }
 
 // rotate the pairs held as (a, b); inv = -1 for the transposed rotation
@@ -105,26 +129,33 @@ struct Params {
   float* part;
 };
 
-// NJ chunks per lane; G = lanes per head
-template <typename T, typename TW, int PV, int NJ, int HB, bool INTER, bool BWD, bool WEIGHT>
+// NJ chunks per lane; G = lanes per head; RAG: lanes may share pairs (Chunk::skip)
+template <typename T, typename TW, int PV, int NJ, int HB, bool INTER, bool BWD, bool WEIGHT, bool RAG>
 __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
   const int which = blockIdx.x >= P.side[1].blk0 ? 1 : 0;
   const Side S = P.side[which];
-  const int lane = threadIdx.x % G, group = threadIdx.x / G, groups = kThreads / G;
-  const int d = P.d, half = P.rot >> 1, chunks = (d >> 1) / PV;
+  const int wl = threadIdx.x & 63, gpw = 64 / G, lane = wl % G, first = wl - lane;
+  const int group = (threadIdx.x >> 6) * gpw + wl / G, groups = kThreads / 64 * gpw;
+  const bool pow2 = (G & (G - 1)) == 0, live = wl < gpw * G;  // the wave's last 64 % G lanes have no group
+  const int d = P.d, half = P.rot >> 1;
+  const int chunks = INTER ? cdiv_pv<PV>(d >> 1) : cdiv_pv<PV>(half) + cdiv_pv<PV>((d - P.rot) >> 1);
   const T* X = (const T*)S.x;
   const T* GY = (const T*)S.g;
   T* O = (T*)S.o;
 
-  int o1[NJ], o2[NJ];
+  int o1[NJ], o2[NJ], p0[NJ], skip[NJ];
   bool on[NJ];
   float w1[NJ][PV], w2[NJ][PV];
   float dw1[BWD && WEIGHT ? NJ : 1][PV], dw2[BWD && WEIGHT ? NJ : 1][PV];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int c = lane + G * j;
-    on[j] = c < chunks;
-    chunk_offsets<PV, INTER>(on[j] ? c : 0, d, P.rot, o1[j], o2[j]);
+    on[j] = live && c < chunks;
+    const Chunk ch = chunk_of<PV, INTER>(on[j] ? c : 0, d, P.rot);
+    o1[j] = ch.o1;
+    o2[j] = ch.o2;
+    p0[j] = ch.p0;
+    skip[j] = RAG ? ch.skip : 0;
     if constexpr (WEIGHT) {
       load<TW, PV>(w1[j], (const TW*)S.w + o1[j]);
       load<TW, PV>(w2[j], (const TW*)S.w + o2[j]);
@@ -137,7 +168,10 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
 
   const float inv_d = 1.f / (float)d;
   const int64_t step = (int64_t)S.blocks * groups;
-  for (int64_t task = (int64_t)(blockIdx.x - S.blk0) * groups + group; task < S.tasks; task += step) {
+  for (int64_t t0 = (int64_t)(blockIdx.x - S.blk0) * groups; t0 < S.tasks; t0 += step) {
+    // whole waves stay in the loop (the group sums shuffle); lanes past the tasks redo the last and store nothing
+    const bool work = live && t0 + group < S.tasks;
+    const int64_t task = min(t0 + group, S.tasks - 1);
     const int64_t tok = task / S.sub;
     const int sub = (int)(task - tok * S.sub);
     const int64_t i0 = tok / P.n1, i1 = tok - i0 * P.n1;
@@ -155,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
       const int head = sub + S.sub * h;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        if (on[j] && head < S.heads) {
+        if (on[j] && work && head < S.heads) {
           load<T, PV>(a[h][j], xt + head * S.xsh + o1[j]);
           load<T, PV>(b[h][j], xt + head * S.xsh + o2[j]);
           if constexpr (BWD) {
@@ -174,16 +208,15 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
     float cs[NJ][PV], sn[NJ][PV];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int p0 = PV * (lane + G * j);
-      if (p0 + PV <= half) {
-        load<float, PV>(cs[j], cr + p0);
-        load<float, PV>(sn[j], sr + p0);
+      if (p0[j] + PV <= half) {
+        load<float, PV>(cs[j], cr + p0[j]);
+        load<float, PV>(sn[j], sr + p0[j]);
       } else {
 #pragma unroll
         for (int i = 0; i < PV; ++i) {
-          const bool in = p0 + i < half;
-          cs[j][i] = in ? cr[p0 + i] : 1.f;
-          sn[j][i] = in ? sr[p0 + i] : 0.f;
+          const bool in = p0[j] + i < half;
+          cs[j][i] = in ? cr[p0[j] + i] : 1.f;
+          sn[j][i] = in ? sr[p0[j] + i] : 0.f;
         }
       }
     }
@@ -194,8 +227,14 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int i = 0; i < PV; ++i) ss += a[h][j][i] * a[h][j][i] + b[h][j][i] * b[h][j][i];
-      for (int o = G >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        for (int i = 0; i < PV; ++i) {
+          // interleaved: entry i of a | b is element 2p + i, pair i / 2 and PV / 2 + i / 2
+          const float qa = a[h][j][i] * a[h][j][i], qb = b[h][j][i] * b[h][j][i];
+          if constexpr (!RAG) ss += qa + qb;
+          else if constexpr (INTER) ss += (i / 2 >= skip[j] ? qa : 0.f) + (PV / 2 + i / 2 >= skip[j] ? qb : 0.f);
+          else ss += i >= skip[j] ? qa + qb : 0.f;
+        }
+      ss = group_sum(ss, G, pow2, first);
       float r = rsqrtf(ss * inv_d + P.eps);
       r = ok ? r : __builtin_nanf("");
       if constexpr (!BWD) {
@@ -211,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
             }
           }
           rotate<PV, INTER>(a[h][j], b[h][j], cs[j], sn[j], 1.f);
-          if (on[j] && head < S.heads) {
+          if (on[j] && work && head < S.heads) {
             store<T, PV>(ot + head * S.osh + o1[j], a[h][j]);
             store<T, PV>(ot + head * S.osh + o2[j], b[h][j]);
           }
@@ -228,18 +267,20 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
             if constexpr (WEIGHT) {
               // rows past the heads and lanes past the head size hold zeros (0 * NaN only where
               // the position itself is bad)
-              if (on[j] && head < S.heads) {
+              if (on[j] && work && head < S.heads) {
                 dw1[j][i] += ga[h][j][i] * a[h][j][i];
                 dw2[j][i] += gb[h][j][i] * b[h][j][i];
               }
               ga[h][j][i] *= w1[j][i];
               gb[h][j][i] *= w2[j][i];
             }
-            dot += ga[h][j][i] * a[h][j][i] + gb[h][j][i] * b[h][j][i];
+            const float qa = ga[h][j][i] * a[h][j][i], qb = gb[h][j][i] * b[h][j][i];
+            if constexpr (!RAG) dot += qa + qb;
+            else if constexpr (INTER) dot += (i / 2 >= skip[j] ? qa : 0.f) + (PV / 2 + i / 2 >= skip[j] ? qb : 0.f);
+            else dot += i >= skip[j] ? qa + qb : 0.f;
           }
         }
-        for (int o = G >> 1; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-        dot *= inv_d;
+        dot = group_sum(dot, G, pow2, first) * inv_d;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -247,7 +288,7 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
             a[h][j][i] = r * (ga[h][j][i] - a[h][j][i] * dot);
             b[h][j][i] = r * (gb[h][j][i] - b[h][j][i] * dot);
           }
-          if (on[j] && head < S.heads) {
+          if (on[j] && work && head < S.heads) {
             store<T, PV>(ot + head * S.osh + o1[j], a[h][j]);
             store<T, PV>(ot + head * S.osh + o2[j], b[h][j]);
           }
@@ -257,15 +298,16 @@ __global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
   }
 
   if constexpr (BWD && WEIGHT) {
-    // [groups][d] image: groups * d <= 256 / G * 2 PV NJ G floats
+    // [groups][d] image: at most 256 / G * 2 PV NJ G floats
     extern __shared__ __attribute__((aligned(16))) float red[];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if (on[j]) {
 #pragma unroll
         for (int i = 0; i < PV; ++i) {
-          red[group * d + o1[j] + i] = dw1[j][i];
-          red[group * d + o2[j] + i] = dw2[j][i];
+          const bool own1 = !RAG || (INTER ? i / 2 : i) >= skip[j], own2 = !RAG || (INTER ? PV / 2 + i / 2 : i) >= skip[j];
+          if (own1) red[group * d + o1[j] + i] = dw1[j][i];
+          if (own2) red[group * d + o2[j] + i] = dw2[j][i];
         }
       }
     }
@@ -306,23 +348,24 @@ __global__ void __launch_bounds__(1024) dw_finalize(const float* __restrict__ pa
 
 struct Plan {
   int pv, g, nj, hb;
+  bool rag;
   int sub[2], blocks[2];
 };
 
-// PV = 8 (16-byte vectors of 16-bit types) wherever no vector crosses the end of the rotated part:
-// interleaved pairs need d % 16 == 0, half-split ones rot % 16 == 0 and (d - rot) % 16 == 0.  Other
-// head sizes take one pair per lane and step.
+// PV = 8 (16-byte vectors of 16-bit types) wherever the rotated part and the rest hold a lane's 8 pairs or
+// nothing (interleaved: the head does); smaller ones take one pair per lane and step.
 inline Plan make_plan(const QkRopeArgs& a, int cus, bool bwd) {
   Plan p{};
-  const bool vec = a.interleaved ? a.d % 16 == 0 : a.rot % 16 == 0 && (a.d - a.rot) % 16 == 0;
+  const int pairs = a.d / 2, half = a.rot / 2, rest = pairs - half;
+  const bool vec = a.interleaved ? pairs >= 8 : (half == 0 || half >= 8) && (rest == 0 || rest >= 8);
   p.pv = vec ? 8 : 1;
-  const int chunks = a.d / 2 / p.pv;
-  p.g = 1;
-  while (p.g < chunks && p.g < 64) p.g <<= 1;
+  const int chunks = !vec ? pairs : a.interleaved ? cdiv_pv<8>(pairs) : cdiv_pv<8>(half) + cdiv_pv<8>(rest);
+  p.rag = vec && (a.interleaved ? pairs % 8 != 0 : half % 8 != 0 || rest % 8 != 0);
+  p.g = chunks < 64 ? chunks : 64;
   p.nj = (chunks + p.g - 1) / p.g;
   if (p.nj == 3) p.nj = 4;
   const int64_t tokens = a.n0 * a.n1;
-  const int groups = kThreads / p.g;
+  const int groups = kThreads / 64 * (64 / p.g);
   // HB heads share one load of the cosines; one head each when there are too few heads to fill
   // the chip (single-token calls: latency counts, not loads)
   const int64_t rows = tokens * (a.hq + a.hk);
@@ -339,7 +382,7 @@ inline Plan make_plan(const QkRopeArgs& a, int cus, bool bwd) {
   return p;
 }
 
-template <typename T, typename TW, int PV, int NJ, int HB, bool INTER, bool BWD, bool WEIGHT>
+template <typename T, typename TW, int PV, int NJ, int HB, bool INTER, bool BWD, bool WEIGHT, bool RAG>
 void launch(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
   Params P{};
   const int64_t tokens = a.n0 * a.n1;
@@ -361,8 +404,8 @@ void launch(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
   P.ps1 = a.ps1;
   P.eps = a.eps;
   P.part = a.part;
-  const size_t lds = BWD && WEIGHT ? (size_t)(kThreads / p.g) * a.d * sizeof(float) : 0;
-  hipLaunchKernelGGL((qk_kernel<T, TW, PV, NJ, HB, INTER, BWD, WEIGHT>), dim3(p.blocks[0] + p.blocks[1]),
+  const size_t lds = BWD && WEIGHT ? (size_t)(kThreads / 64 * (64 / p.g)) * a.d * sizeof(float) : 0;
+  hipLaunchKernelGGL((qk_kernel<T, TW, PV, NJ, HB, INTER, BWD, WEIGHT, RAG>), dim3(p.blocks[0] + p.blocks[1]),
                      dim3(kThreads), lds, s, P, p.g);
   if (BWD && WEIGHT)
     hipLaunchKernelGGL((dw_finalize<TW>), dim3((a.d + 15) / 16, 2), dim3(1024), 0, s, a.part, p.blocks[0], p.blocks[1],
@@ -371,20 +414,23 @@ void launch(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
 
 template <typename T, typename TW, bool BWD, bool WEIGHT>
 void dispatch_shape(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
-  auto inter = [&](auto pv, auto nj, auto hb) {
+  auto inter = [&](auto pv, auto nj, auto hb, auto rag) {
     constexpr int PV = decltype(pv)::value, NJ = decltype(nj)::value, HB = decltype(hb)::value;
-    if (a.interleaved) launch<T, TW, PV, NJ, HB, true, BWD, WEIGHT>(a, p, s);
-    else launch<T, TW, PV, NJ, HB, false, BWD, WEIGHT>(a, p, s);
+    constexpr bool RAG = decltype(rag)::value;
+    if (a.interleaved) launch<T, TW, PV, NJ, HB, true, BWD, WEIGHT, RAG>(a, p, s);
+    else launch<T, TW, PV, NJ, HB, false, BWD, WEIGHT, RAG>(a, p, s);
   };
-  auto hb = [&](auto pv, auto nj) {
-    if (p.hb == 1) inter(pv, nj, std::integral_constant<int, 1>{});
-    else inter(pv, nj, std::integral_constant<int, BWD ? 2 : 4>{});
+  auto hb = [&](auto pv, auto nj, auto rag) {
+    if (p.hb == 1) inter(pv, nj, std::integral_constant<int, 1>{}, rag);
+    else inter(pv, nj, std::integral_constant<int, BWD ? 2 : 4>{}, rag);
   };
   using I1 = std::integral_constant<int, 1>;
-  if (p.pv == 8) hb(std::integral_constant<int, 8>{}, I1{});
-  else if (p.nj == 1) hb(I1{}, I1{});
-  else if (p.nj == 2) hb(I1{}, std::integral_constant<int, 2>{});
-  else hb(I1{}, std::integral_constant<int, 4>{});
+  using I8 = std::integral_constant<int, 8>;
+  if (p.pv == 8 && p.rag) hb(I8{}, I1{}, std::true_type{});
+  else if (p.pv == 8) hb(I8{}, I1{}, std::false_type{});
+  else if (p.nj == 1) hb(I1{}, I1{}, std::false_type{});
+  else if (p.nj == 2) hb(I1{}, std::integral_constant<int, 2>{}, std::false_type{});
+  else hb(I1{}, std::integral_constant<int, 4>{}, std::false_type{});
 }
 
 template <bool BWD>
