@@ -12,11 +12,12 @@
 // mean is one sum over the group's lanes.  Half-split pairs load the vectors i and i + rot/2, interleaved ones
 // 2 PV consecutive elements.  Where the rotated part or the rest is no multiple of PV pairs, its last lane
 // starts earlier: the pairs it shares with its neighbour are computed (and stored) twice and counted
-// once, which keeps every access a vector (head 80 with 34 rotated, 32768 x 16 heads bf16: XX us forward and YY
+// once, which keeps every access a vector (head 80 with 34 rotated, 32768 x 16 heads bf16: 39 us forward and 77
 // backward; one pair a lane and step took 103 and 215).
-// A group takes HB heads of its token (cosines and sines are loaded once for them, all HB loads are in flight
-// together); neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole
-// cache lines.  Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums
+// A forward group takes two heads of its token (cosines and sines are loaded once for them, their loads are
+// in flight together), a backward group one, and the registers stay within four waves a SIMD: 51 and 81 us at
+// 32768 x 16 heads x 128 bf16, 5.2 and 4.9 TB/s (four heads and two: 56 and 90; a plain copy runs at 4.9).
+// Neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole cache lines.  Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums
 // belong to one tensor for the whole kernel.
 // dw: fp32 per lane over the persistent loop, per block through LDS, then a fixed-order column sum
 // over the blocks (no atomics: the same inputs give the same bits).
@@ -29,6 +30,7 @@ namespace apex_amd {
 namespace qkr {
 
 constexpr int kThreads = 256;
+constexpr int kHeads = 2;  // HB of the forward
 
 // PV elements at p, any element alignment (gfx950 takes 16-byte accesses at 2-byte addresses)
 template <typename T, int PV> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T e[PV]; };
@@ -131,7 +133,7 @@ struct Params {
 
 // NJ chunks per lane; G = lanes per head; RAG: lanes may share pairs (Chunk::skip)
 template <typename T, typename TW, int PV, int NJ, int HB, bool INTER, bool BWD, bool WEIGHT, bool RAG>
-__global__ void __launch_bounds__(kThreads) qk_kernel(const Params P, int G) {
+__global__ void __launch_bounds__(kThreads, BWD ? 4 : RAG ? 3 : 4) qk_kernel(const Params P, int G) {
   const int which = blockIdx.x >= P.side[1].blk0 ? 1 : 0;
   const Side S = P.side[which];
   const int wl = threadIdx.x & 63, gpw = 64 / G, lane = wl % G, first = wl - lane;
@@ -366,12 +368,11 @@ inline Plan make_plan(const QkRopeArgs& a, int cus, bool bwd) {
   if (p.nj == 3) p.nj = 4;
   const int64_t tokens = a.n0 * a.n1;
   const int groups = kThreads / 64 * (64 / p.g);
-  // HB heads share one load of the cosines; one head each when there are too few heads to fill
-  // the chip (single-token calls: latency counts, not loads)
+  // one head each when there are too few to fill the chip (single-token calls: latency counts, not loads)
   const int64_t rows = tokens * (a.hq + a.hk);
-  p.hb = rows >= (int64_t)cus * groups * 4 ? (bwd ? 2 : 4) : 1;
+  p.hb = !bwd && rows >= (int64_t)cus * groups * 4 ? kHeads : 1;
   const int heads[2] = {a.hq, a.hk};
-  int64_t cap = (int64_t)cus * 8;  // persistent; four a CU made the backward 257 us at 32768 x 40 x 128 (222)
+  const int64_t cap = (int64_t)cus * 8;  // persistent: the backward's blocks each leave a partial row
   for (int i = 0; i < 2; ++i) {
     p.sub[i] = (heads[i] + p.hb - 1) / p.hb;
     const int64_t need = (tokens * p.sub[i] + groups - 1) / groups;
@@ -421,8 +422,10 @@ void dispatch_shape(const QkRopeArgs& a, const Plan& p, hipStream_t s) {
     else launch<T, TW, PV, NJ, HB, false, BWD, WEIGHT, RAG>(a, p, s);
   };
   auto hb = [&](auto pv, auto nj, auto rag) {
-    if (p.hb == 1) inter(pv, nj, std::integral_constant<int, 1>{}, rag);
-    else inter(pv, nj, std::integral_constant<int, BWD ? 2 : 4>{}, rag);
+    if constexpr (!BWD) {
+      if (p.hb > 1) return inter(pv, nj, std::integral_constant<int, kHeads>{}, rag);
+    }
+    inter(pv, nj, std::integral_constant<int, 1>{}, rag);
   };
   using I1 = std::integral_constant<int, 1>;
   using I8 = std::integral_constant<int, 8>;
