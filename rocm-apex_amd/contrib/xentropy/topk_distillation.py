@@ -10,7 +10,7 @@ of student ``logits`` ``[rows, classes]`` and the ``top`` largest logits the tea
 them).  An entry with a negative index is no entry (a row may keep fewer); a row without entries (or
 whose teacher logits are all -inf) has zero loss and zero gradient, whatever its logits hold.  Entries naming
 one class twice both count.  An index past the classes makes the row's loss and gradient NaN.  The
-teacher is a constant: it takes no gradient.
+teacher is a constant: it takes no gradient.  The loss is differentiable once (``create_graph`` is refused).
 
 GPU: the gfx950 kernels of ``csrc/xentropy/topk_distill.hip`` (the logits are read once forward and
 once backward, in place for any row pitch); CPU: the same math in torch.  Like

@@ -4,7 +4,8 @@
 likewise), ``weight2`` is ``[out, intermediate]``; the activation is ``silu`` or ``gelu`` (tanh form, as
 :class:`FusedDenseGeluDense`).  fp16 / bf16 GPU tensors with widths that are multiples of 8 run the gfx950
 kernels of ``csrc/gemm/gated_ffn.hip``: both projections, the activation and the product are one MFMA
-kernel, the backward's ``[da | du]`` another, and no operand is transposed or concatenated in memory.
+kernel, the backward's ``[da | du]`` another, and no operand is transposed or concatenated in memory
+(differentiable once: ``create_graph`` is refused).
 Other types and widths (CPU, fp32, odd sizes) run the same math in torch, as the other fused dense layers."""
 import torch
 from torch import nn

@@ -63,7 +63,8 @@ def fused_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps=1e-6, 
     ``rotary_dim`` may be smaller than the head, the rest of the head is then normed only.
     ``positions``: integers, broadcastable to the token axes; a position outside the table makes that
     token's output (and gradients) NaN.  ``interleaved`` rotates the pairs ``(2i, 2i + 1)`` instead of
-    ``(i, i + rotary_dim / 2)``.  The head size is even, up to 512 on the GPU."""
+    ``(i, i + rotary_dim / 2)``.  The head size is even, up to 512 on the GPU, where the operator is
+    differentiable once (``create_graph`` is refused)."""
     if q.dim() not in (3, 4) or q.dim() != k.dim() or q.shape[:-2] != k.shape[:-2] or q.size(-1) != k.size(-1):
         raise ValueError(f"q and k must be [..., heads, d] with the same one or two token axes and d, got "
                          f"{tuple(q.shape)} and {tuple(k.shape)}")

@@ -147,7 +147,8 @@ def test_cpu_refusals():
 # ------------------------------------------------------------------------------------------- GPU
 # one token; odd row counts around the tiles; widths that end inside a 16-byte k step, a 64-deep tile,
 # a tile; splits over the tokens; several tiles each way
-SHAPES = [(1, 8, 8, 8), (1, 256, 136, 64), (3, 64, 128, 72), (17, 72, 264, 136), (33, 512, 1000, 256), (64, 128, 64, 40),
+SHAPES = [(1, 8, 8, 8), (1, 256, 136, 64), (3, 64, 128, 72), (16, 104, 5504, 8), (17, 72, 264, 136), (24, 5512, 24, 16),
+          (32, 264, 136, 520), (33, 512, 1000, 256), (64, 128, 64, 40),
           (65, 320, 520, 328), (127, 200, 344, 96), (257, 264, 712, 520), (700, 256, 384, 128), (2100, 136, 200, 72),
           (4097, 64, 72, 264)]
 
@@ -190,6 +191,21 @@ def test_gpu_no_tokens():
     assert y.shape == (0, 48)
     y.sum().backward()
     assert x.grad.shape == (0, 64) and all((t.grad == 0).all() for t in (w1, b1, w2, b2))
+
+
+@pytest.mark.gpu
+def test_gpu_offsets_past_32_bits():
+    # [tokens, 2 x intermediate] has 2.3e9 elements; its last rows against 64 bits
+    x, w1, _, w2, _, _ = _inputs("cuda", 8, 64, 8192, 64, torch.bfloat16, False)
+    m = 140000
+    x = torch.randn(m, 64, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    dy = torch.randn(m, 64, device="cuda").to(torch.bfloat16)
+    y = fused_dense_gated_dense_function(x, w1, None, w2, None)
+    dx, = torch.autograd.grad(y, x, dy)
+    tail = slice(m - 40, m)
+    want = _exact(x[tail], w1, None, w2, None, "silu", dy[tail])
+    _close(y[tail], *want["y"], 64, "y")
+    _close(dx[tail], *want["dx"], 64, "dx")
 
 
 @pytest.mark.gpu

@@ -90,7 +90,7 @@ def _check_case(c, eps, inter):
 SHAPES = [  # lead, hq, hk, d, rot
     ((5,), 4, 4, 64, 64), ((3, 2), 4, 2, 128, 128), ((1, 1), 1, 1, 2, 2), ((7,), 3, 1, 80, 32),
     ((1, 9), 5, 5, 72, 72), ((2, 3), 6, 2, 96, 0), ((4,), 2, 2, 256, 64), ((2, 2), 2, 1, 34, 18), ((3,), 7, 7, 512, 512),
-    ((2,), 1, 3, 130, 66),
+    ((2,), 1, 3, 130, 66), ((3,), 2, 1, 400, 398), ((5,), 3, 2, 200, 8), ((31,), 7, 2, 144, 52), ((2, 9), 3, 1, 176, 160),
 ]
 
 
@@ -233,7 +233,7 @@ def test_gpu_other_stream_and_captured_graph():
 
     def step():
         o = fused_qk_norm_rope(q, k, qw, kw, cos, sin, pos)
-        return list(o) + list(torch.autograd.grad(o, [q, k, qw, kw], (gq, gk)))
+        return [t.detach() for t in o] + list(torch.autograd.grad(o, [q, k, qw, kw], (gq, gk)))
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())

@@ -227,7 +227,7 @@ def test_gpu_other_stream_captured_graph_and_repeatability():
 
     def step():
         loss = SoftmaxTopKDistillationLoss.apply(x, z, idx, 2.0, True)
-        return loss, torch.autograd.grad(loss, x, w)[0]
+        return loss.detach(), torch.autograd.grad(loss, x, w)[0]
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
