@@ -22,6 +22,10 @@
 // The gate and up columns of a tile are dealt so that a wave holds both for the same outputs (its
 // first BN/4 columns are rows of Wg, its last BN/4 the same rows of Wu): act(a) u is taken on the
 // accumulators, in fp32, and rounded once.
+// Measured (bf16, us of kernel): 8192 x 4096 -> 11008: gated 1230-1310 (1.13-1.2 PFLOP/s, and 0.7 GB written);
+// [da | du] 720-760; the plain products 555-660 (NT, NN, TN; 1.13-1.33 PFLOP/s, at the card's power limit:
+// 1.6 GHz).  The 128 x 64 eight-wave tiles of gemm_mfma.hip take 1296, 855 and 617-871 there.
+//
 // The MFMAs compute the transposed tile (the n operand first), which leaves four consecutive n of one
 // row in a lane: the epilogue parks them in LDS with 8- / 16-byte writes and every global access of it
 // is a 16-byte vector of consecutive columns.
@@ -570,6 +574,7 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 // through LDS by DMA, whole 64 U byte runs of a row at a time: read like the weights, 64 bytes of 16 rows a
 // load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels instead of 24).  The waves' partial tiles
 // meet in LDS in a fixed order, where the block's epilogue (bias, activation, product) runs in fp32.
+// One token at 4096 -> 11008 -> 4096: 31 + 17 us, 5.8 and 5.3 TB/s of weights.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
