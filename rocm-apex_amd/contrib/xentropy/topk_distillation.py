@@ -10,7 +10,7 @@ of student ``logits`` ``[rows, classes]`` and the ``top`` largest logits the tea
 them).  An entry with a negative index is no entry (a row may keep fewer); a row without entries (or
 whose teacher logits are all -inf) has zero loss and zero gradient, whatever its logits hold.  Entries naming
 one class twice both count.  An index past the classes makes the row's loss and gradient NaN.  The
-teacher is a constant: it takes no gradient.  The loss is differentiable once (``create_graph`` is refused).
+teacher is a constant: it takes no gradient.  Temperatures are between 1e-15 and 1e15.  The loss is differentiable once (``create_graph`` is refused).
 
 GPU: the gfx950 kernels of ``csrc/xentropy/topk_distill.hip`` (the logits are read once forward and
 once backward, in place for any row pitch); CPU: the same math in torch.  Like
@@ -39,8 +39,9 @@ def _check(logits, teacher_logits, teacher_indices, temperature):
                         f"{teacher_logits.dtype} and {teacher_indices.dtype}")
     if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
         raise ValueError("the teacher's logits and indices must be on the logits' device")
-    if not 0 < temperature < float("inf"):
-        raise ValueError(f"the temperature must be positive and finite, got {temperature}")
+    # 1 / T and T^2 are fp32 factors of the kernels' exponents and losses
+    if not 1e-15 <= temperature <= 1e15:
+        raise ValueError(f"the temperature must be between 1e-15 and 1e15, got {temperature}")
     if _native.use_native(logits):
         if logits.dtype not in (torch.float16, torch.bfloat16, torch.float32):
             raise TypeError(f"fp16, bf16 or fp32 logits expected on the GPU, got {logits.dtype}")

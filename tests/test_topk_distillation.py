@@ -143,6 +143,25 @@ def test_cpu_refusals():
     _refusals("cpu")
 
 
+def _temperature_range(dev):
+    """1 / T or T^2 past fp32's range would make every loss NaN: refused; inside, the limits T -> 0 and T -> inf
+    hold: one-hot distributions that agree, and terms of size 1 / T that vanish next to their coefficient."""
+    f = SoftmaxTopKDistillationLoss.apply
+    x = torch.tensor([[0.0, 3.0, 1.0, -2.0]], device=dev, requires_grad=True)
+    z, i = torch.tensor([[2.0, 1.0]], device=dev), torch.tensor([[1, 2]], device=dev)
+    for t in (1e-46, 1e-16, 1e16, 1e39, 1e-320):
+        with pytest.raises(ValueError):
+            f(x, z, i, t)
+    loss = f(x, z, i, 1e-15, True)
+    grad, = torch.autograd.grad(loss.sum(), x)
+    assert loss.item() == 0 and (grad == 0).all()
+    assert torch.isfinite(f(x, z, i, 1e15, True)).all()
+
+
+def test_cpu_temperature_range():
+    _temperature_range("cpu")
+
+
 # ------------------------------------------------------------------------------------------- GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,v,top", SHAPES + [(2, 50257, 33), (1100, 3001, 5), (1, 131072, 1024), (1025, 257, 256)])
@@ -183,6 +202,11 @@ def test_gpu_refusals():
         f(x, i[:, :2].float(), i[:, :2].cpu())
     with pytest.raises(TypeError):
         f(x.double(), i[:, :2].float(), i[:, :2])
+
+
+@pytest.mark.gpu
+def test_gpu_temperature_range():
+    _temperature_range("cuda")
 
 
 @pytest.mark.gpu
