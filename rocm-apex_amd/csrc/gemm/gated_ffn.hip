@@ -62,7 +62,8 @@ struct Params {
 // LDS-DMA of 16 bytes a lane to dst + 16 lane.  Written in assembly: behind the builtin the compiler makes
 // every transposing LDS read wait for all DMA in flight (it cannot tell their LDS ranges apart), and the
 // tile that should land during the next four k steps would be waited out in the first.  The waits are
-// the caller's: s_waitcnt vmcnt(0) before the barrier that opens the tile.  No register is written.
+// the caller's: an s_waitcnt vmcnt before the barrier that opens a tile, counted so that only younger tiles'
+// DMA stays in flight.  No register is written, and the compiler's own counts only become stricter.
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void dma(i32x4 r, int voff, uint32_t dst) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know the constraints
@@ -572,7 +573,8 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 // A workgroup owns 16 outputs (16 rows of Wg and of Wu, or of W2) and its NW waves split K; the weights
 // go straight from memory to the MFMA operand (16 rows x 32 k a load), U steps in flight per wave.  x goes
 // through LDS by DMA, whole 64 U byte runs of a row at a time: read like the weights, 64 bytes of 16 rows a
-// load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels instead of 24).  The waves' partial tiles
+// load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels
+// instead of 24).  The waves' partial tiles
 // meet in LDS in a fixed order, where the block's epilogue (bias, activation, product) runs in fp32.
 // One token at 4096 -> 11008 -> 4096: 31 + 17 us, 5.8 and 5.3 TB/s of weights.
 // ---------------------------------------------------------------------------------------------

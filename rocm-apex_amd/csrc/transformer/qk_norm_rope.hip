@@ -17,8 +17,9 @@
 // A forward group takes two heads of its token (cosines and sines are loaded once for them, their loads are
 // in flight together), a backward group one, and the registers stay within four waves a SIMD: 51 and 81 us at
 // 32768 x 16 heads x 128 bf16, 5.2 and 4.9 TB/s (four heads and two: 56 and 90; a plain copy runs at 4.9).
-// Neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole cache lines.  Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums
-// belong to one tensor for the whole kernel.
+// Neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole cache lines.
+// Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums belong to
+// one tensor for the whole kernel.
 // dw: fp32 per lane over the persistent loop, per block through LDS, then a fixed-order column sum
 // over the blocks (no atomics: the same inputs give the same bits).
 // Positions outside the table give NaN rows (the table is never read past its end).
@@ -83,7 +84,7 @@ __device__ __forceinline__ float group_sum(float v, int G, bool pow2, int first)
   return t;
 }
 
-// rotate the pairs held as (a, b); inv = -1 for the transposed rotation
+// rotate the pairs held as (a, b); dir = -1 for the transposed rotation
 template <int PV, bool INTER>
 __device__ __forceinline__ void rotate(float (&a)[PV], float (&b)[PV], const float (&c)[PV], const float (&s)[PV],
                                        float dir) {

@@ -5,10 +5,10 @@
 //   loss = T^2 sum_k t_k (log t_k - log q_{j_k})          (T^2 KL(t || q); 0 for a row without entries)
 //   dx_v = g T (q_v - sum_k t_k [j_k = v])
 //
-// Both passes are bound by the logits' bytes (8192 x 50304 bf16: 5.3 TB/s forward, 4.8-5.2 backward): the forward reads them once (running maximum and
-// rescaled sum per lane over 8-element vectors, in base 2 with 1/T folded into its scale), the
-// backward reads them once and writes the gradient once.  Rows of any pitch and alignment (odd
-// vocabularies) take the same 16-byte accesses at element-aligned addresses.
+// Both passes are bound by the logits' bytes (8192 x 50304 bf16: 5.3 TB/s forward, 4.8-5.2 backward): the
+// forward reads them once (running maximum and rescaled sum per lane over 8-element vectors, in base 2
+// with 1/T folded into its scale), the backward reads them once and writes the gradient once.  Rows of
+// any pitch and alignment (odd vocabularies) take the same 16-byte accesses at element-aligned addresses.
 // A row is one workgroup when there are rows enough to fill the chip; fewer rows are split over
 // workgroups, (maximum, sum) pairs of the parts joined in a fixed order by a second launch.
 // In the backward the workgroup that wrote a class's dense value also writes the teacher's
@@ -151,7 +151,10 @@ kd_fwd_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const fl
   for (; v + 24 * kThreads + 8 <= c1; v += 32 * kThreads) {  // four vectors in flight
     Pack8<T> w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = STREAM ? stream8(x + v + 8 * kThreads * i) : *reinterpret_cast<const Pack8<T>*>(x + v + 8 * kThreads * i);
+    for (int i = 0; i < 4; ++i) {
+      const T* p = x + v + 8 * kThreads * i;
+      w[i] = STREAM ? stream8(p) : *reinterpret_cast<const Pack8<T>*>(p);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float r[8];
@@ -294,7 +297,8 @@ void dispatch(const TopkDistillArgs& a, F&& f) {
 }
 
 inline void check(const TopkDistillArgs& a) {
-  if (a.rows < 0 || a.rows > kDistillMaxRows || a.classes < 1 || a.classes > INT_MAX - (1 << 16) || a.top < 0 || a.top > kDistillMaxTop)
+  if (a.rows < 0 || a.rows > kDistillMaxRows || a.classes < 1 || a.classes > INT_MAX - (1 << 16) || a.top < 0 ||
+      a.top > kDistillMaxTop)
     throw std::runtime_error("topk_distill: sizes out of range");
 }
 
