@@ -161,20 +161,18 @@ __device__ __forceinline__ s16x8 frag(const uint16_t* tile, int rowbase, int kk,
   }
 }
 
-// act(x), and its derivative in d
+// act(x) = x s, and its derivative in d; s = 1 / (1 + e^-y) with y = x for SiLU and 2 k0 (x + k1 x^3) for the
+// tanh form of GeLU.  The epilogues' instructions count, since the matrix units are idle meanwhile: e^-y
+// is one exp2 with log2(e) in y's constants, and d = s + x s (1 - s) y'.
 template <int ACT>
 __device__ __forceinline__ float activate(float x, float& d) {
-  if constexpr (ACT == kGateSilu) {
-    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-x));
-    d = s * (1.f + x * (1.f - s));
-    return x * s;
-  } else {
-    // tanh-GeLU as x sigmoid(2 v), v = k0 (x + k1 x^3)
-    const float k0 = 0.7978845608028654f, k1 = 0.044715f;
-    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-2.f * k0 * (x + k1 * x * x * x)));
-    d = s + 2.f * x * s * (1.f - s) * k0 * (1.f + 3.f * k1 * x * x);
-    return x * s;
-  }
+  constexpr float kLog2e = 1.4426950408889634f, k0 = 0.7978845608028654f, k1 = 0.044715f;
+  const float x2 = x * x;
+  const float y = ACT == kGateSilu ? -kLog2e * x : x * fmaf(-2.f * k0 * k1 * kLog2e, x2, -2.f * k0 * kLog2e);
+  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y));
+  const float p = x * s, q = p * (1.f - s);
+  d = ACT == kGateSilu ? s + q : fmaf(q, fmaf(6.f * k0 * k1, x2, 2.f * k0), s);
+  return p;
 }
 
 template <typename T>
@@ -185,10 +183,20 @@ __device__ __forceinline__ void load4(float (&r)[4], const T* p) {
   r[2] = to_f(T{(uint16_t)w.y});
   r[3] = to_f(T{(uint16_t)(w.y >> 16)});
 }
+// rounded to nearest even, two at a time (one by one the compiler adds a shift and an or to each pair)
 template <typename T>
 __device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
-  return make_uint2((uint32_t)from_f<T>(v[0]).x | (uint32_t)from_f<T>(v[1]).x << 16,
-                    (uint32_t)from_f<T>(v[2]).x | (uint32_t)from_f<T>(v[3]).x << 16);
+  using E = std::conditional_t<std::is_same_v<T, bf16_t>, __bf16, _Float16>;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef E e16x2 __attribute__((ext_vector_type(2)));
+  return make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[0], v[1]}), e16x2)),
+                    __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{v[2], v[3]}), e16x2)));
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  const uint2 lo = pack4<T>({v[0], v[1], v[2], v[3]}), hi = pack4<T>({v[4], v[5], v[6], v[7]});
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
 // Pre-activations are kept for the backward as the upper 24 bits of their fp32 value (15 bits of
@@ -559,8 +567,8 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
         }
         if (gr < P.M && gc < P.N) {
           T* o = out + (int64_t)gr * P.ldc + gc;
-          Vec8<T>::store(o, da);
-          Vec8<T>::store(o + P.N, du);
+          *reinterpret_cast<uint4*>(o) = pack8<T>(da);
+          *reinterpret_cast<uint4*>(o + P.N) = pack8<T>(du);
         }
       }
       __syncthreads();
