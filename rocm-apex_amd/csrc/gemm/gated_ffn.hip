@@ -163,13 +163,14 @@ __device__ __forceinline__ s16x8 frag(const uint16_t* tile, int rowbase, int kk,
 
 // act(x) = x s, and its derivative in d; s = 1 / (1 + e^-y) with y = x for SiLU and 2 k0 (x + k1 x^3) for the
 // tanh form of GeLU.  The epilogues' instructions count, since the matrix units are idle meanwhile: e^-y
-// is one exp2 with log2(e) in y's constants, and d = s + x s (1 - s) y'.
+// is one exp2 (of z) with log2(e) in y's constants, and d = s + x s (1 - s) y'.  x^2 stops at 1e4: s is 0 or 1
+// long before, and an infinite y' would make 0 y' NaN.
 template <int ACT>
 __device__ __forceinline__ float activate(float x, float& d) {
   constexpr float kLog2e = 1.4426950408889634f, k0 = 0.7978845608028654f, k1 = 0.044715f;
-  const float x2 = x * x;
-  const float y = ACT == kGateSilu ? -kLog2e * x : x * fmaf(-2.f * k0 * k1 * kLog2e, x2, -2.f * k0 * kLog2e);
-  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y));
+  const float x2 = fminf(x * x, 1e4f);
+  const float z = ACT == kGateSilu ? -kLog2e * x : x * fmaf(-2.f * k0 * k1 * kLog2e, x2, -2.f * k0 * kLog2e);
+  const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z));
   const float p = x * s, q = p * (1.f - s);
   d = ACT == kGateSilu ? s + q : fmaf(q, fmaf(6.f * k0 * k1, x2, 2.f * k0), s);
   return p;

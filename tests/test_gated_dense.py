@@ -226,6 +226,30 @@ def test_gpu_extreme_activations(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 40])
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_gpu_square_of_a_pre_activation_past_fp32(kind, m):
+    """a = -+2^67: act' is 0 and 1 there, though a^2 is no fp32 number.  Powers of two, each the single term of
+    its sum: every value is exact."""
+    x, w1, w2 = torch.zeros(m, 8), torch.zeros(16, 8), torch.zeros(8, 8)
+    x[1, 0], x[2, 0], x[:, 1] = -2.0 ** 33, 2.0 ** 33, 1.0
+    w1[0, 0], w1[8, 1], w2[0, 0] = 2.0 ** 34, 1.0, 1.0  # the first feature: a = 2^34 x0, u = 1
+    x, w1, w2 = (t.to("cuda", torch.bfloat16).requires_grad_(True) for t in (x, w1, w2))
+    y = fused_dense_gated_dense_function(x, w1, None, w2, None, kind)
+    dy = torch.zeros_like(y)
+    dy[1:3, 0] = 1.0
+    dx, dw1, dw2 = torch.autograd.grad(y, (x, w1, w2), dy)
+    want_y, want_dx, want_dw1, want_dw2 = torch.zeros(m, 8), torch.zeros(m, 8), torch.zeros(16, 8), torch.zeros(8, 8)
+    want_y[2, 0] = 2.0 ** 67
+    want_dx[2, 0], want_dx[2, 1] = 2.0 ** 34, 2.0 ** 67       # da = act'(a) u = 1, du = act(a)
+    want_dw1[0, 0], want_dw1[0, 1] = 2.0 ** 33, 1.0           # da x of row 2
+    want_dw1[8, 0], want_dw1[8, 1] = 2.0 ** 100, 2.0 ** 67    # du x
+    want_dw2[0, 0] = 2.0 ** 67
+    for got, want in ((y, want_y), (dx, want_dx), (dw1, want_dw1), (dw2, want_dw2)):
+        assert torch.equal(got.detach().cpu().float(), want)
+
+
+@pytest.mark.gpu
 def test_gpu_nan_stays_in_its_row():
     x, w1, b1, w2, b2, dy = _inputs("cuda", 300, 72, 136, 64, torch.bfloat16, False)
     want = fused_dense_gated_dense_function(x, w1, None, w2, None).detach()
