@@ -185,6 +185,22 @@ def test_gpu_layouts_and_leading_axes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("with1,with2", [(False, False), (True, False), (False, True), (True, True)])
+def test_gpu_frozen_leaves(with1, with2):
+    # either bias alone, and any single leaf that takes a gradient: the same bits as with all of them
+    x, w1, b1, w2, b2, dy = _inputs("cuda", 70, 64, 96, 48, torch.bfloat16, True)
+    b1, b2 = b1 if with1 else None, b2 if with2 else None
+    given = [x, w1, b1, w2, b2]
+    leaves = [t for t in given if t is not None]
+    full = torch.autograd.grad(fused_dense_gated_dense_function(*given), leaves, dy)
+    for t, want in zip(leaves, full):
+        only = [v if v is t or v is None else v.detach() for v in given]
+        y = fused_dense_gated_dense_function(*only)
+        y.backward(dy)
+        assert torch.equal(t.grad, want)
+
+
+@pytest.mark.gpu
 def test_gpu_no_tokens():
     x, w1, b1, w2, b2, _ = _inputs("cuda", 0, 64, 96, 48, torch.bfloat16, True)
     y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)

@@ -261,3 +261,36 @@ def test_gpu_no_second_derivative():
     qo, _ = fused_qk_norm_rope(q, k, qw, kw, cos, sin, pos)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(qo, q, gq, create_graph=True)
+
+
+def _frozen(dev):
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(dev)
+    q, k, qw, kw, gq, gk = rnd(2, 9, 4, 24), rnd(2, 9, 2, 24), rnd(24), rnd(24), rnd(2, 9, 4, 24), rnd(2, 9, 2, 24)
+    pos = torch.arange(9, device=dev)
+    tables = rotary_tables(16, 16, device=dev)
+    given = [t.requires_grad_(True) for t in (q, k, qw, kw)]
+    for weights in (True, False):
+        leaves = given if weights else given[:2]
+        pick = lambda ts: list(ts) if weights else list(ts[:2]) + [None, None]
+        full = torch.autograd.grad(fused_qk_norm_rope(*pick(given), *tables, pos), leaves, (gq, gk))
+        for t, want in zip(leaves, full):
+            only = pick([v if v is t else v.detach() for v in given])
+            outs = fused_qk_norm_rope(*only, *tables, pos)
+            pairs = [(o, go) for o, go in zip(outs, (gq, gk)) if o.requires_grad]
+            got, = torch.autograd.grad([o for o, _ in pairs], t, [go for _, go in pairs])
+            assert torch.equal(got, want)
+    # one output alone: the other's input takes no gradient from it
+    qo, _ = fused_qk_norm_rope(*given, *tables, pos)
+    dq, dk = torch.autograd.grad(qo, [q, k], gq, allow_unused=True)
+    want, = torch.autograd.grad(fused_qk_norm_rope(*given, *tables, pos), [q], (gq, gk))
+    assert torch.equal(dq, want) and (dk is None or (dk == 0).all())
+
+
+def test_cpu_frozen_leaves():
+    _frozen("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_frozen_leaves():
+    _frozen("cuda")
