@@ -583,9 +583,9 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 // go straight from memory to the MFMA operand (16 rows x 32 k a load), U steps in flight per wave.  x goes
 // through LDS by DMA, whole 64 U byte runs of a row at a time: read like the weights, 64 bytes of 16 rows a
 // load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels
-// instead of 24).  The waves' partial tiles
+// instead of 24, now 22).  The waves' partial tiles
 // meet in LDS in a fixed order, where the block's epilogue (bias, activation, product) runs in fp32.
-// One token at 4096 -> 11008 -> 4096: 31 + 17 us, 5.8 and 5.3 TB/s of weights.
+// One token at 4096 -> 11008 -> 4096: 31 + 16 us, 5.8 and 5.7 TB/s of weights.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -715,17 +715,17 @@ void launch_few(const FfnArgs& g, hipStream_t s) {
   hipLaunchKernelGGL((ffn_few_kernel<T, GATED, ACT, TM, NW>), dim3((unsigned)((g.n + 15) / 16)), dim3(NW * 64), lds, s, P);
 }
 
-// 16 waves a workgroup where there are too few outputs for two workgroups a CU, else 8
+// Eight waves a workgroup; sixteen, with half the groups of steps one after the other, for a long second product
+// of two token fragments.  us with 8 and 16 waves, K -> outputs: 24 rows 5504 -> 2048: 9.5, 11.1; 24 rows
+// 8192 -> 4096: 17.6, 18.8; 32 rows 11008 -> 4096: 22.5, 20.0; 20 rows 16384 -> 8192: 76, 65.  One row 11008 ->
+// 4096: 15.8, 17.0; gated, 24 rows 2048 -> 5504: 12.3, 12.9; 20 rows 8192 -> 16384: 101, 104.
 template <typename T, bool GATED, int ACT>
-void launch_few_tm(const FfnArgs& g, int cus, hipStream_t s) {
-  const bool wide = (g.n + 15) / 16 < 2 * cus;
-  auto go = [&](auto tm) {
-    constexpr int TM = decltype(tm)::value;
-    if (wide) launch_few<T, GATED, ACT, TM, 16>(g, s);
-    else launch_few<T, GATED, ACT, TM, 8>(g, s);
-  };
-  if (g.m <= 16) go(std::integral_constant<int, 1>{});
-  else go(std::integral_constant<int, 2>{});
+void launch_few_tm(const FfnArgs& g, hipStream_t s) {
+  if (g.m <= 16) return launch_few<T, GATED, ACT, 1, 8>(g, s);
+  if constexpr (!GATED) {
+    if (g.k > 8192) return launch_few<T, GATED, ACT, 2, 16>(g, s);
+  }
+  launch_few<T, GATED, ACT, 2, 8>(g, s);
 }
 
 // sum of the split-K partials (fixed order) + bias
@@ -832,7 +832,8 @@ bool ffn_supported(const FfnArgs& g) {
   }
 }
 
-// up to 32 rows of a k-major x k-major product
+// Up to 32 rows of a k-major x k-major product.  4096 -> 11008 -> 4096, us: 32 rows 36 + 25; 33 rows, on the
+// tiles, 49 + 28 (which 128 rows also take: 52 + 31).
 static bool ffn_few(const FfnArgs& g) { return g.m <= ffn::kFewRows && g.a_kmajor && g.b_kmajor; }
 
 int64_t ffn_workspace_floats(const FfnArgs& g, int cus) {
@@ -846,9 +847,9 @@ void ffn_gemm(const FfnArgs& g, int cus, hipStream_t s) {
   if (ffn_few(g)) {
     dispatch_16(g.dtype, [&](auto tag) {
       using T = typename decltype(tag)::type;
-      if (g.op != kFfnGated) ffn::launch_few_tm<T, false, 0>(g, cus, s);
-      else if (g.act == kGateSilu) ffn::launch_few_tm<T, true, kGateSilu>(g, cus, s);
-      else ffn::launch_few_tm<T, true, kGateGelu>(g, cus, s);
+      if (g.op != kFfnGated) ffn::launch_few_tm<T, false, 0>(g, s);
+      else if (g.act == kGateSilu) ffn::launch_few_tm<T, true, kGateSilu>(g, s);
+      else ffn::launch_few_tm<T, true, kGateGelu>(g, s);
     }, "gated_ffn");
     check_launch("gated_ffn");
     return;

@@ -162,6 +162,13 @@ def test_gpu_block(m, k, f, n, kind, bias, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,f,n", [(17, 16, 8200, 24), (32, 24, 11016, 40), (16, 8, 8200, 16)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gpu_few_rows_of_a_long_second_product(m, k, f, n, dtype):
+    _check(*_inputs("cuda", m, k, f, n, dtype, True), "silu")
+
+
+@pytest.mark.gpu
 def test_gpu_layouts_and_leading_axes():
     x, w1, b1, w2, b2, dy = _inputs("cuda", 60, 64, 96, 48, torch.bfloat16, True)
     want = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
