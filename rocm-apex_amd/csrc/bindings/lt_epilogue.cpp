@@ -131,7 +131,7 @@ std::mutex g_plan_mu;
 // APEX_AMD_LT_TUNE=0: take the heuristic's first answer (deterministic across ranks / runs);
 // default: time the top kTop answers once per problem on its first (non-captured) call and keep
 // the fastest — the single-answer heuristic picked a 32 x 32-tile BGRADB kernel ~10x slower than
-// the plain GEMM at the GPT-2 shapes (VERDICT r03 weak #8).  Every candidate is screened with
+// the plain GEMM at the GPT-2 shapes.  Every candidate is screened with
 // hipblaslt_ext::matmulIsAlgoSupported (and its workspace need against ours) before it is
 // launched at all.  The pick is recorded as an index into the screened list: plan_choices() /
 // set_plan_choice() let the Python side make it identical on every rank of a tensor-parallel
@@ -139,10 +139,8 @@ std::mutex g_plan_mu;
 // from different kernels on different ranks.
 constexpr int kTop = 8;
 // APEX_AMD_LT_TUNE_MAX_DIM=<n> limits timing to problems with every dimension <= n (default: no
-// limit).  Round 4 capped it at 16384: before the support screen existed, one unscreened candidate
-// at 32768 tokens (and at m = 200704) made hipBLASLt fail to initialise its kernel ("Could not
-// initialize Tensile host") and crash the process (tools/gpu_r04ab.sh).  With the screen, the
-// uncapped timing runs every one of those shapes (profiles/r06/lt_probe_uncapped_r06v.log).
+// limit): without the support screen, candidates at 32768 tokens (and at m = 200704) made hipBLASLt
+// fail to initialise its kernel ("Could not initialize Tensile host") and end the process.
 int64_t tune_max_dim() {
   static const int64_t v = [] {
     const char* e = std::getenv("APEX_AMD_LT_TUNE_MAX_DIM");
