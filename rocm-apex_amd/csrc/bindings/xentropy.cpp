@@ -60,8 +60,7 @@ void distill_setup(DistillHold& h, const at::Tensor& logits, const at::Tensor& t
               "topk_distill: teacher logits and indices must be [rows, top <= ", kDistillMaxTop, "] on the logits' device");
   TORCH_CHECK(ti.scalar_type() == at::kLong || ti.scalar_type() == at::kInt,
               "topk_distill: teacher indices must be int64 or int32");
-  TORCH_CHECK(logits.size(1) < (int64_t(1) << 30) && logits.size(0) <= kDistillMaxRows,
-              "topk_distill: too many rows or classes");
+  TORCH_CHECK(logits.size(1) < (int64_t(1) << 30), "topk_distill: too many classes");
   TORCH_CHECK(temperature > 0, "topk_distill: the temperature must be positive");
   // rows of any pitch are read in place; other layouts are copied
   h.x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();

@@ -6,8 +6,7 @@
 
 namespace apex_amd {
 
-constexpr int kDistillMaxTop = 1024;              // teacher entries of a row
-constexpr int64_t kDistillMaxRows = (1 << 24) - 1;  // a launch has fewer than 2^32 threads
+constexpr int kDistillMaxTop = 1024;  // teacher entries of a row
 
 struct TopkDistillArgs {
   const void* logits;           // [rows][classes], rows `pitch` elements apart

@@ -297,9 +297,17 @@ void dispatch(const TopkDistillArgs& a, F&& f) {
 }
 
 inline void check(const TopkDistillArgs& a) {
-  if (a.rows < 0 || a.rows > kDistillMaxRows || a.classes < 1 || a.classes > INT_MAX - (1 << 16) || a.top < 0 ||
-      a.top > kDistillMaxTop)
+  if (a.rows < 0 || a.classes < 1 || a.classes > INT_MAX - (1 << 16) || a.top < 0 || a.top > kDistillMaxTop)
     throw std::runtime_error("topk_distill: sizes out of range");
+}
+
+// A launch has fewer than 2^32 threads an axis: more rows than these take another one.
+constexpr int64_t kLaunchRows = ((int64_t(1) << 32) - 1) / kThreads;
+
+// f(row0, rows) for each launch
+template <typename F>
+void launches(int64_t rows, F&& f) {
+  for (int64_t r0 = 0; r0 < rows; r0 += kLaunchRows) f(r0, (unsigned)(rows - r0 < kLaunchRows ? rows - r0 : kLaunchRows));
 }
 
 }  // namespace kd
@@ -320,17 +328,22 @@ void topk_distill_fwd(const TopkDistillArgs& a, float* losses, float* stats, flo
   kd::dispatch(a, [&](auto tag, auto itag) {
     using T = typename decltype(tag)::type;
     using TI = typename decltype(itag)::type;
-    auto go = [&](auto kern) {
-      hipLaunchKernelGGL(kern, dim3((unsigned)a.rows, p), dim3(kd::kThreads), p > 1 ? 0 : lds, s, (const T*)a.logits,
-                         a.pitch, a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top, c, a.temperature,
-                         losses, (float2*)stats, p > 1 ? (float2*)parts : (float2*)nullptr, chunk);
-    };
-    if (a.rows * a.classes * (int64_t)sizeof(T) > kd::kLastCache) go(kd::kd_fwd_kernel<T, TI, true>);
-    else go(kd::kd_fwd_kernel<T, TI, false>);
-    if (p > 1)
-      hipLaunchKernelGGL((kd::kd_join_kernel<T, TI>), dim3((unsigned)a.rows), dim3(kd::kThreads), lds, s,
-                         (const T*)a.logits, a.pitch, a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top,
-                         c, a.temperature, losses, (float2*)stats, (const float2*)parts, p);
+    kd::launches(a.rows, [&](int64_t r0, unsigned rows) {
+      const T* x = (const T*)a.logits + r0 * a.pitch;
+      const float* tz = a.teacher_logits + r0 * a.top;
+      const TI* ti = (const TI*)a.teacher_indices + r0 * a.top;
+      float2* st = (float2*)stats + r0;
+      float2* pt = p > 1 ? (float2*)parts + r0 * p : nullptr;
+      auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3(rows, p), dim3(kd::kThreads), p > 1 ? 0 : lds, s, x, a.pitch, a.classes, tz, ti,
+                           a.top, c, a.temperature, losses + r0, st, pt, chunk);
+      };
+      if (a.rows * a.classes * (int64_t)sizeof(T) > kd::kLastCache) go(kd::kd_fwd_kernel<T, TI, true>);
+      else go(kd::kd_fwd_kernel<T, TI, false>);
+      if (p > 1)
+        hipLaunchKernelGGL((kd::kd_join_kernel<T, TI>), dim3(rows), dim3(kd::kThreads), lds, s, x, a.pitch, a.classes,
+                           tz, ti, a.top, c, a.temperature, losses + r0, st, (const float2*)pt, p);
+    });
   });
   check_launch("topk_distill forward");
 }
@@ -345,10 +358,13 @@ void topk_distill_bwd(const TopkDistillArgs& a, const float* grad_loss, int64_t 
   kd::dispatch(a, [&](auto tag, auto itag) {
     using T = typename decltype(tag)::type;
     using TI = typename decltype(itag)::type;
-    hipLaunchKernelGGL((kd::kd_bwd_kernel<T, TI>), dim3((unsigned)a.rows, p), dim3(kd::kThreads),
-                       (size_t)2 * a.top * sizeof(float), s, grad_loss, grad_loss_stride, (const T*)a.logits, a.pitch,
-                       a.classes, a.teacher_logits, (const TI*)a.teacher_indices, a.top, c, a.temperature,
-                       (const float2*)stats, (T*)grad, chunk);
+    kd::launches(a.rows, [&](int64_t r0, unsigned rows) {
+      hipLaunchKernelGGL((kd::kd_bwd_kernel<T, TI>), dim3(rows, p), dim3(kd::kThreads),
+                         (size_t)2 * a.top * sizeof(float), s, grad_loss + r0 * grad_loss_stride, grad_loss_stride,
+                         (const T*)a.logits + r0 * a.pitch, a.pitch, a.classes, a.teacher_logits + r0 * a.top,
+                         (const TI*)a.teacher_indices + r0 * a.top, a.top, c, a.temperature, (const float2*)stats + r0,
+                         (T*)grad + r0 * a.classes, chunk);
+    });
   });
   check_launch("topk_distill backward");
 }

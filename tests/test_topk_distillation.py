@@ -278,3 +278,16 @@ def test_gpu_no_second_derivative():
     x, z, idx, w = _case("cuda", 5, 99, 4, torch.float32)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(SoftmaxTopKDistillationLoss.apply(x, z, idx, 1.0, True), x, w, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_gpu_more_rows_than_a_launch_has():
+    # 512 threads a row: 2^32 threads are 2^23 rows.  Rows on both sides of it against 64 bits.
+    rows, v = (1 << 23) + 5, 3
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, v, device="cuda", generator=g).to(torch.bfloat16).requires_grad_(True)
+    z = torch.randn(rows, 2, device="cuda", generator=g)
+    idx = torch.tensor([2, 0], dtype=torch.int32, device="cuda").repeat(rows, 1)
+    idx[-1] = -1
+    w = torch.rand(rows, device="cuda", generator=g)
+    _check(x, z, idx, w, 2.0)
