@@ -50,27 +50,35 @@ def _check(logits, teacher_logits, teacher_indices, temperature):
 
 
 def _torch_teacher(teacher_logits, teacher_indices, temperature, classes, acc):
-    """(t, log t, index clamped to the classes, rows with entries, rows with a bad index)."""
+    """(t, T log t, index clamped to the classes, rows with entries, rows with a bad index)."""
     live = (teacher_indices >= 0) & (teacher_indices < classes)
     bad = (teacher_indices >= classes).any(-1)
-    z = (teacher_logits.to(acc) / temperature).masked_fill(~live, float("-inf"))
+    z = teacher_logits.to(acc).masked_fill(~live, float("-inf"))
     if z.size(1) == 0:
         return z, z, teacher_indices.long(), bad, bad
     zm = z.amax(-1, keepdim=True)
-    zm = torch.where(torch.isinf(zm) & (zm < 0), torch.zeros_like(zm), zm)
-    total = torch.exp(z - zm).sum(-1, keepdim=True)
+    z = z - torch.where(torch.isinf(zm) & (zm < 0), torch.zeros_like(zm), zm)
+    total = torch.exp(z / temperature).sum(-1, keepdim=True)
     some = total.squeeze(-1) != 0
-    logt = z - zm - torch.log(torch.where(total != 0, total, torch.ones_like(total)))
-    t = torch.where(some[:, None], torch.exp(logt), torch.zeros_like(z))
-    return t, logt, torch.where(live, teacher_indices, torch.zeros_like(teacher_indices)).long(), some, bad
+    total = torch.where(total != 0, total, torch.ones_like(total))
+    t = torch.where(some[:, None], torch.exp(z / temperature) / total, torch.zeros_like(z))
+    tlogt = z - temperature * torch.log(total)
+    return t, tlogt, torch.where(live, teacher_indices, torch.zeros_like(teacher_indices)).long(), some, bad
+
+
+def _torch_student(logits, acc):
+    # the maximum goes first: logits of the type's lowest value over a temperature below 1 are no numbers of acc
+    x = logits.to(acc)
+    return x - x.amax(-1, keepdim=True)
 
 
 def _torch_forward(logits, teacher_logits, teacher_indices, temperature):
     acc = torch.promote_types(logits.dtype, torch.float32)
-    t, logt, idx, some, bad = _torch_teacher(teacher_logits, teacher_indices, temperature, logits.size(1), acc)
-    # log_softmax takes the maximum off first: logits of the type's lowest value keep log(sum)
-    logq = torch.log_softmax(logits.to(acc) / temperature, -1).gather(1, idx)
-    terms = torch.where(t != 0, t * (logt - logq), torch.zeros_like(t)).sum(-1) * temperature ** 2
+    t, tlogt, idx, some, bad = _torch_teacher(teacher_logits, teacher_indices, temperature, logits.size(1), acc)
+    # T log q: log q of such a logit overflows where its term of the loss does not
+    x = _torch_student(logits, acc)
+    tlogq = x.gather(1, idx) - temperature * torch.logsumexp(x / temperature, -1, keepdim=True)
+    terms = torch.where(t != 0, t * (tlogt - tlogq), torch.zeros_like(t)).sum(-1) * temperature
     terms = torch.where(some, terms, torch.zeros_like(terms))
     return terms.masked_fill(bad, float("nan"))
 
@@ -78,7 +86,7 @@ def _torch_forward(logits, teacher_logits, teacher_indices, temperature):
 def _torch_backward(grad_loss, logits, teacher_logits, teacher_indices, temperature):
     acc = torch.promote_types(logits.dtype, torch.float32)
     t, _, idx, some, bad = _torch_teacher(teacher_logits, teacher_indices, temperature, logits.size(1), acc)
-    q = torch.softmax(logits.to(acc) / temperature, -1)
+    q = torch.softmax(_torch_student(logits, acc) / temperature, -1)
     g = (grad_loss.to(acc) * temperature).masked_fill(bad, float("nan"))[:, None]
     dx = g * q.scatter_add(1, idx, -t)
     return torch.where((some | bad)[:, None], dx, torch.zeros_like(dx)).to(logits.dtype)

@@ -29,6 +29,7 @@ namespace kd {
 
 constexpr int kThreads = 512;  // 8192 x 50304 bf16: 182 + 315 us, with 256 threads a row 188 + 338, with 1024 239 + 321
 constexpr int kWaves = kThreads / 64;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int64_t kLastCache = 256ll << 20;  // bytes of the memory-side cache
 
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Pack8 { T e[8]; };
@@ -98,8 +99,8 @@ __device__ __forceinline__ int teacher_entries(const float* __restrict__ z, cons
   return (int)block_max(state, red);
 }
 
-// logits in t -> weights; log2 of them in lt (forward)
-__device__ __forceinline__ void teacher_weights(int top, float c, float* t, float* lt, float* red) {
+// logits in t -> weights; T log of them in lt (forward)
+__device__ __forceinline__ void teacher_weights(int top, float c, float temp, float* t, float* lt, float* red) {
   float m = -INFINITY;
   for (int k = threadIdx.x; k < top; k += kThreads) m = fmaxf(m, t[k]);
   m = block_max(m, red);
@@ -107,28 +108,29 @@ __device__ __forceinline__ void teacher_weights(int top, float c, float* t, floa
   float s = 0.f;
   for (int k = threadIdx.x; k < top; k += kThreads) s += exp2_((t[k] - b) * c);
   s = block_sum(s, red);
-  const float inv = 1.f / s, ls = __builtin_amdgcn_logf(s);
+  const float inv = 1.f / s, ls = temp * kLn2 * __builtin_amdgcn_logf(s);
   for (int k = threadIdx.x; k < top; k += kThreads) {
-    const float y = (t[k] - b) * c;
+    const float y = t[k] - b;
     if (lt != nullptr) lt[k] = y - ls;
-    t[k] = exp2_(y) * inv;
+    t[k] = exp2_(y * c) * inv;
   }
   __syncthreads();
 }
 
-// the row's loss and its (maximum, sum), from the latter (thread 0 writes)
+// The row's loss and its (maximum, sum), from the latter (thread 0 writes).  Its terms are T t (T log t - T log q):
+// log q of a logit at its type's lowest value overflows where its term does not.
 template <typename T>
-__device__ __forceinline__ void row_loss(const T* __restrict__ x, float m, float s, float c, float temp, int state,
-                                         int top, const int* cls, const float* t, const float* lt, float* red,
+__device__ __forceinline__ void row_loss(const T* __restrict__ x, float m, float s, float temp, int state, int top,
+                                         const int* cls, const float* t, const float* lt, float* red,
                                          float* __restrict__ loss, float2* __restrict__ stat) {
-  const float ls = __builtin_amdgcn_logf(s);
+  const float ls = temp * kLn2 * __builtin_amdgcn_logf(s);
   float a = 0.f;
   if (state == 1)
     for (int k = threadIdx.x; k < top; k += kThreads)
-      if (cls[k] >= 0 && t[k] != 0.f) a += t[k] * (lt[k] - ((to_f(x[cls[k]]) - m) * c - ls));
+      if (cls[k] >= 0 && t[k] != 0.f) a += t[k] * (lt[k] - (to_f(x[cls[k]]) - m - ls));
   a = block_sum(a, red);
   if (threadIdx.x == 0) {
-    *loss = state == 2 ? __builtin_nanf("") : temp * temp * 0.6931471805599453f * a;
+    *loss = state == 2 ? __builtin_nanf("") : temp * a;
     *stat = make_float2(m, s);
   }
 }
@@ -191,8 +193,8 @@ kd_fwd_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const fl
   int* cls = (int*)lds;
   float *t = lds + top, *lt = lds + 2 * top;
   const int state = teacher_entries(tz + row * top, ti + row * top, top, classes, cls, t, red);
-  if (state == 1) teacher_weights(top, c, t, lt, red);
-  row_loss(x, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
+  if (state == 1) teacher_weights(top, c, temp, t, lt, red);
+  row_loss(x, m, s, temp, state, top, cls, t, lt, red, losses + row, stats + row);
 }
 
 // join a row's parts (fixed order) and take its loss
@@ -214,8 +216,8 @@ kd_join_kernel(const T* __restrict__ logits, int64_t pitch, int classes, const f
   int* cls = (int*)lds;
   float *t = lds + top, *lt = lds + 2 * top;
   const int state = teacher_entries(tz + row * top, ti + row * top, top, classes, cls, t, red);
-  if (state == 1) teacher_weights(top, c, t, lt, red);
-  row_loss(logits + row * pitch, m, s, c, temp, state, top, cls, t, lt, red, losses + row, stats + row);
+  if (state == 1) teacher_weights(top, c, temp, t, lt, red);
+  row_loss(logits + row * pitch, m, s, temp, state, top, cls, t, lt, red, losses + row, stats + row);
 }
 
 template <typename T, typename TI>
@@ -260,7 +262,7 @@ kd_bwd_kernel(const float* __restrict__ gl, int64_t gl_stride, const T* __restri
   for (int e = tail + threadIdx.x; e < c1; e += kThreads) gx[e] = from_f<T>(pc * exp2_((to_f(x[e]) - b) * c));
   if (state != 1) return;  // NaN everywhere already
   // the weights are taken while the stores above drain; its barriers also order them before the stores below
-  teacher_weights(top, c, t, nullptr, red);
+  teacher_weights(top, c, temp, t, nullptr, red);
   for (int k = threadIdx.x; k < top; k += kThreads) {
     const int j = cls[k];
     if (j < c0 || j >= c1) continue;

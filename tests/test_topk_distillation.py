@@ -291,3 +291,32 @@ def test_gpu_more_rows_than_a_launch_has():
     idx[-1] = -1
     w = torch.rand(rows, device="cuda", generator=g)
     _check(x, z, idx, w, 2.0)
+
+
+def _lowest_values(dev, dtype, temp):
+    """Logits at the lowest value of their type, the student's or the teacher's: x / T is no fp32 number there
+    below T = 1, and log q (up to 3.4e38 / T) overflows where T^2 t log q does not."""
+    low = torch.finfo(torch.float32).min
+    x = torch.tensor([[0.0, 1.0, 2.0, -1.0, 0.5]], device=dev).repeat(5, 1).to(dtype)
+    x[0] = torch.finfo(dtype).min                 # every class
+    x[1, 2:] = torch.finfo(dtype).min             # masked ones, none of the teacher's
+    x[3, 0] = torch.finfo(dtype).min              # one that the teacher names
+    z = torch.tensor([[0.5, 0.5]], device=dev).repeat(5, 1)
+    z[2] = low                                    # a teacher that knows no difference
+    z[4, 0] = low                                 # ... and one that excludes an entry
+    idx = torch.tensor([[0, 1]], device=dev).repeat(5, 1)
+    w = torch.tensor([0.5, 0.75, 1.0, 1.25, 1.5], device=dev)
+    _check(x.requires_grad_(True), z, idx, w, temp)
+
+
+@pytest.mark.parametrize("temp", [0.25, 1.0, 1.5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_cpu_lowest_values(dtype, temp):
+    _lowest_values("cpu", dtype, temp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("temp", [0.25, 1.0, 1.5])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_gpu_lowest_values(dtype, temp):
+    _lowest_values("cuda", dtype, temp)
