@@ -116,6 +116,12 @@ struct MtaIO {
 template <typename Op, int D, int I, typename... Ts>
 struct ListIO {
   using T = typename TypeAt<I, Ts...>::type;
+  // The fp16 copy is the rounding of the fp32 value that its master list gets: kept apart from the
+  // arithmetic before it, which the compiler would fold into one conversion of the unrounded sum.
+  static __device__ __forceinline__ float fp32_value(float v) {
+    if constexpr (std::is_same<T, f16_t>::value) asm("" : "+v"(v));
+    return v;
+  }
   static __device__ __forceinline__ void load_vec(float (&r)[D][kVec], void* const (&base)[D], int i) {
     if constexpr ((Op::kRead >> I) & 1u) MtaIO<T>::load(r[I], reinterpret_cast<const T*>(base[I]) + i);
     else {
@@ -125,18 +131,11 @@ struct ListIO {
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::load_vec(r, base, i);
   }
   static __device__ __forceinline__ void store_vec(const float (&r)[D][kVec], void* const (&base)[D], int i) {
-    if constexpr (((Op::kWrite >> I) & 1u) && std::is_same<T, f16_t>::value) {
-      // the fp16 copy is the rounding of the fp32 value that its master list gets: kept apart from the
-      // arithmetic before it, which the compiler would fold into one conversion of the unrounded sum
+    if constexpr ((Op::kWrite >> I) & 1u) {
       float v[kVec];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        v[k] = r[I][k];
-        asm("" : "+v"(v[k]));
-      }
+      for (int k = 0; k < kVec; ++k) v[k] = fp32_value(r[I][k]);
       MtaIO<T>::store(reinterpret_cast<T*>(base[I]) + i, v);
-    } else if constexpr ((Op::kWrite >> I) & 1u) {
-      MtaIO<T>::store(reinterpret_cast<T*>(base[I]) + i, r[I]);
     }
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::store_vec(r, base, i);
   }
@@ -146,7 +145,7 @@ struct ListIO {
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::load_one(r, base, i);
   }
   static __device__ __forceinline__ void store_one(const float (&r)[D][1], void* const (&base)[D], int i) {
-    if constexpr ((Op::kWrite >> I) & 1u) reinterpret_cast<T*>(base[I])[i] = from_f<T>(r[I][0]);
+    if constexpr ((Op::kWrite >> I) & 1u) reinterpret_cast<T*>(base[I])[i] = from_f<T>(fp32_value(r[I][0]));
     if constexpr (I + 1 < D) ListIO<Op, D, I + 1, Ts...>::store_one(r, base, i);
   }
   static __device__ __forceinline__ void set_base(void* (&base)[D], const MtaMeta& m, int t, int64_t start) {

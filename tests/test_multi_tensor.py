@@ -285,3 +285,23 @@ def test_table_hit_during_capture_is_pinned_gpu():
     for x, y in zip(xs, ys):
         torch.testing.assert_close(y, x * 2.0)
     assert noop.item() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["sgd", "adam"])
+@pytest.mark.parametrize("n,offset", [((1 << 22) + 5, 0), ((1 << 22) + 5, 1), (7, 0)])
+def test_fp16_copy_is_the_rounding_of_its_master(op, n, offset):
+    """Whatever a list's alignment: the copy is master.half(), bit by bit, in the vectors, in a tail of 1 to 7
+    elements and in misaligned lists, which are scalar throughout."""
+    g = torch.Generator().manual_seed(n + offset)
+    mk = lambda dt=torch.float32: [torch.randn(n + offset, generator=g).to("cuda", dt)[offset:]]
+    grad, w, m, v, copy = mk(), mk(), mk(), [mk()[0].abs()], mk(torch.float16)
+    for step in range(1, 4):
+        if op == "sgd":
+            amp_C.multi_tensor_sgd(CHUNK, _noop("cuda"), [grad, w, m, copy], 0.01, 0.9, 0.0, 0.1, False, step == 1,
+                                   False, 1.0)
+        else:
+            amp_C.multi_tensor_adam_capturable(CHUNK, _noop("cuda"), [grad, w, m, v, copy], torch.full((1,), 0.01).cuda(),
+                                               0.9, 0.999, 1e-8, torch.full((1,), float(step)).cuda(), 1, 1, 0.01,
+                                               torch.ones(1).cuda())
+        assert torch.equal(copy[0], w[0].half())
