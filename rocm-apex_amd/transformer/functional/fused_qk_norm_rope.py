@@ -32,7 +32,7 @@ def _torch_qk_norm_rope(x, weight, cos, sin, positions, eps, interleaved):
     xf = x.to(acc)
     n = xf * torch.rsqrt((xf * xf).mean(-1, keepdim=True) + eps)
     if weight is not None:
-        n = n * weight.to(acc)
+        n = n * weight.to(acc).reshape(-1)
     rot = 2 * cos.size(1)
     bad = (positions < 0) | (positions >= cos.size(0))
     pos = torch.where(bad, torch.zeros_like(positions), positions)

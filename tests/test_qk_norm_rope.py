@@ -294,3 +294,24 @@ def test_cpu_frozen_leaves():
 @pytest.mark.gpu
 def test_gpu_frozen_leaves():
     _frozen("cuda")
+
+
+def _weight_layouts(dev):
+    # weights of d entries in any shape, the head size among the head counts: each entry belongs to its element
+    q, k, qw, kw, cos, sin, pos, gq, gk = _case(dev, (3,), 4, 4, 4, 4, False, torch.float32, torch.float32, False)
+    leaves = [q, k, qw, kw]
+    want = fused_qk_norm_rope(q, k, qw, kw, cos, sin, pos)
+    want_g = torch.autograd.grad(want, leaves, (gq, gk))
+    for shape in ((1, 4), (4, 1), (2, 2)):
+        got = fused_qk_norm_rope(q, k, qw.view(shape), kw.view(shape), cos, sin, pos)
+        got_g = torch.autograd.grad(got, leaves, (gq, gk))
+        assert all(torch.equal(a, b) for a, b in zip(got + got_g, want + want_g))
+
+
+def test_cpu_weight_layouts():
+    _weight_layouts("cpu")
+
+
+@pytest.mark.gpu
+def test_gpu_weight_layouts():
+    _weight_layouts("cuda")
