@@ -358,6 +358,26 @@ void bind_gemm(pybind11::module_& root) {
   gf.attr("ACT_SILU") = (int)kGateSilu;
   gf.attr("ACT_GELU") = (int)kGateGelu;
   gf.def("gated_ffn", &gated_ffn);
+  // (tile width, splits of K) of the six products, in order: gated, down, dW2, [da | du], dW1, dx
+  gf.def("plans", [](int64_t m, int64_t k, int64_t f, int64_t n, int64_t cus) {
+    struct Product { int op; bool a, b; int64_t m, n, k; };
+    const Product ps[] = {{kFfnGated, true, true, m, f, k},  {kFfnPlain, true, true, m, n, f},
+                          {kFfnPlain, false, false, n, f, m}, {kFfnDGated, true, false, m, f, n},
+                          {kFfnPlain, false, false, 2 * f, k, m}, {kFfnPlain, true, false, m, k, 2 * f}};
+    std::vector<std::pair<int, int>> out;
+    for (const Product& p : ps) {
+      FfnArgs g{};
+      g.op = p.op;
+      g.a_kmajor = p.a;
+      g.b_kmajor = p.b;
+      g.m = (int)p.m;
+      g.n = (int)p.n;
+      g.k = (int)p.k;
+      const FfnPlan r = ffn_plan(g, (int)cus);
+      out.emplace_back(r.bn, r.splits);
+    }
+    return out;
+  });
 
   auto fd = root.def_submodule("fused_dense_cuda", "fused dense (GEMM + bias [+ GeLU]) on gfx950 MFMA");
   fd.def("linear_bias_forward", [](at::Tensor input, at::Tensor weight, OT bias) {

@@ -836,9 +836,14 @@ bool ffn_supported(const FfnArgs& g) {
 // tiles, 49 + 28 (which 128 rows also take: 52 + 31).
 static bool ffn_few(const FfnArgs& g) { return g.m <= ffn::kFewRows && g.a_kmajor && g.b_kmajor; }
 
-int64_t ffn_workspace_floats(const FfnArgs& g, int cus) {
-  if (ffn_few(g)) return 0;
+FfnPlan ffn_plan(const FfnArgs& g, int cus) {
+  if (ffn_few(g)) return {0, 1};
   const ffn::Plan p = ffn::make_plan(g, cus);
+  return {p.bn, p.splits};
+}
+
+int64_t ffn_workspace_floats(const FfnArgs& g, int cus) {
+  const FfnPlan p = ffn_plan(g, cus);
   return p.splits > 1 ? (int64_t)p.splits * g.m * g.n : 0;
 }
 

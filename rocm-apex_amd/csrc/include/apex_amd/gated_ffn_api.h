@@ -35,6 +35,9 @@ struct FfnArgs {
 
 // the kernels' conditions: sizes, strides and bases in 16-byte vectors
 bool ffn_supported(const FfnArgs& g);
+// the kernels that a product takes: tile width (0: the few-row kernel) and splits of K, from op, sizes and layouts
+struct FfnPlan { int bn, splits; };
+FfnPlan ffn_plan(const FfnArgs& g, int cus);
 int64_t ffn_workspace_floats(const FfnArgs& g, int cus);
 void ffn_gemm(const FfnArgs& g, int cus, hipStream_t s);
 

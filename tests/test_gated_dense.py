@@ -337,3 +337,39 @@ def test_gpu_no_second_derivative():
     y = fused_dense_gated_dense_function(x, w1, b1, w2, b2)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(y, x, dy, create_graph=True)
+
+
+# Sizes whose products take the 256-wide tile, several K tiles deep and with ragged edges (SHAPES are 128-wide
+# throughout): (tile width, splits of K) of gated, down, dW2, [da | du], dW1 and dx on 256 compute units
+W, N = (256, 1), (128, 1)
+PLANNED = [((777, 712, 4104, 264), [W, (128, 8), N, N, N, (128, 10)]),
+           ((4099, 264, 520, 2056), [N, W, (128, 5), N, (128, 8), N]),
+           ((523, 264, 4104, 2056), [N, (128, 5), W, N, N, (128, 15)]),
+           ((4099, 264, 5512, 264), [W, (128, 5), (256, 5), N, N, (128, 5)]),
+           ((4107, 520, 2056, 520), [N, (128, 3), (128, 5), W, (128, 3), (128, 3)]),
+           ((523, 2600, 1544, 264), [N, (128, 3), N, N, W, (128, 4)]),
+           ((4099, 2056, 520, 264), [N, N, (128, 8), N, (128, 3), W]),
+           ((777, 2056, 5512, 264), [W, (128, 10), N, N, N, (256, 7)]),
+           ((2057, 2600, 5512, 2056), [W, (256, 3), W, W, W, (256, 2)])]
+
+
+def _plans(shape, cus):
+    native = pytest.importorskip("apex._native")
+    if not native.available():
+        pytest.skip("native extension not built")
+    return native.require("gated_ffn").gated_ffn.plans(*shape, cus)
+
+
+@pytest.mark.parametrize("shape,plans", PLANNED)
+def test_cpu_plans(shape, plans):
+    """The sizes below stay on the kernels that they are there for."""
+    assert _plans(shape, 256) == plans
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,plans", PLANNED)
+@pytest.mark.parametrize("kind,bias,dtype", [("silu", True, torch.bfloat16), ("gelu", False, torch.bfloat16),
+                                             ("silu", False, torch.float16), ("gelu", True, torch.float16)])
+def test_gpu_wide_tiles(shape, plans, kind, bias, dtype):
+    assert _plans(shape, torch.cuda.get_device_properties(0).multi_processor_count) == plans
+    _check(*_inputs("cuda", *shape, dtype, bias), kind)
