@@ -315,3 +315,18 @@ def test_cpu_weight_layouts():
 @pytest.mark.gpu
 def test_gpu_weight_layouts():
     _weight_layouts("cuda")
+
+
+# Tokens enough that every lane takes several heads (2048 blocks of 4 (64 / G) groups, G lanes a head, two heads a
+# forward group), odd head counts (a group's second head past the last); half-split pairs: groups of 6, 5, 5, 32,
+# 12, 64 and 64 lanes
+LOOPED = [(14500, 80, 34), (17400, 72, 72), (17400, 72, 40), (2900, 512, 512), (7300, 24, 8), (1500, 200, 8), (1500, 400, 398)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,d,rot", LOOPED)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32),
+                                          (torch.float16, torch.float16), (torch.bfloat16, None)])
+def test_gpu_more_heads_than_groups(tokens, d, rot, inter, dtype, wdtype):
+    _check_case(_case("cuda", (tokens,), 7, 3, d, rot, inter, dtype, wdtype, True), 1e-6, inter)
