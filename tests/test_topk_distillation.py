@@ -320,3 +320,27 @@ def test_cpu_lowest_values(dtype, temp):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_gpu_lowest_values(dtype, temp):
     _lowest_values("cuda", dtype, temp)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_gpu_streamed_logits(dtype):
+    # past 256 MiB the forward streams the logits; an odd vocabulary, so that rows start inside vectors
+    v, top = 131073, 16
+    rows = (260 << 20) // (v * torch.finfo(dtype).bits // 8) + 1
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = (3 * torch.randn(rows, v, device="cuda", generator=g)).to(dtype)
+    idx = torch.randint(0, v, (rows, top), device="cuda", generator=g)
+    idx[:, 0], idx[:, 1] = v - 1, 0               # the row's ends
+    z = 3 * torch.randn(rows, top, device="cuda", generator=g)
+    w = torch.rand(rows, device="cuda", generator=g) + 0.5
+    loss = SoftmaxTopKDistillationLoss.apply(x.requires_grad_(True), z, idx, 2.0, True)
+    grad, = torch.autograd.grad(loss, x, w)
+    eps = torch.finfo(dtype).eps
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -126
+    for r in range(0, rows, 100):                 # the bounds of _check, in blocks of rows
+        b = slice(r, r + 100)
+        want, mag, dx, dmag = _exact(x[b], z[b], idx[b], 2.0, w[b])
+        log_sum = 2.0 ** 2 * (v / 256 + 16) * 2.0 ** -24
+        assert ((loss[b].double() - want).abs() <= 2.0 ** -17 * mag + 2.0 ** -24 * want.abs() + log_sum).all()
+        assert ((grad[b].double() - dx).abs() <= eps / 2 * 1.01 * dx.abs() + 2.0 ** -16 * dmag + tiny).all()
