@@ -373,3 +373,8 @@ def test_cpu_plans(shape, plans):
 def test_gpu_wide_tiles(shape, plans, kind, bias, dtype):
     assert _plans(shape, torch.cuda.get_device_properties(0).multi_processor_count) == plans
     _check(*_inputs("cuda", *shape, dtype, bias), kind)
+
+
+@pytest.mark.gpu
+def test_gpu_autocast_bf16():
+    _autocast("cuda", torch.bfloat16)
