@@ -35,6 +35,7 @@
 #include "apex_amd/dispatch.h"
 #include "apex_amd/gated_ffn_api.h"
 #include "apex_amd/mfma.h"
+#include "apex_amd/tile_order.h"
 
 namespace apex_amd {
 namespace ffn {
@@ -80,20 +81,6 @@ __device__ __forceinline__ i32x4 rsrc(const uint16_t* p, int64_t elems) {
 
 __device__ __forceinline__ uint32_t lds_addr(const uint16_t* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint16_t*)p;
-}
-
-// XCD-aware, bijective remap of the linear workgroup id (each XCD gets a contiguous band), then
-// GROUP_M-grouped tile order
-__device__ __forceinline__ void tile_coords(int tiles_m, int tiles_n, int& bm, int& bn) {
-  const int nwg = tiles_m * tiles_n, orig = blockIdx.x;
-  const int xcd = orig % 8, q = nwg / 8, r = nwg % 8;
-  const int wgid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + orig / 8;
-  constexpr int GROUP_M = 8;
-  const int group = wgid / (GROUP_M * tiles_n);
-  const int first_m = group * GROUP_M;
-  const int gm = min(tiles_m - first_m, GROUP_M);
-  bm = first_m + (wgid % (GROUP_M * tiles_n)) % gm;
-  bn = (wgid % (GROUP_M * tiles_n)) / gm;
 }
 
 // One operand's tile of R rows x 64 k on its way into LDS, R / 32 instructions of 1 KB a wave.
@@ -330,7 +317,7 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
   const int wm = wave >> 1, wn = wave & 1;
   const int tiles_m = (P.M + BM - 1) / BM, tiles_n = (P.N + HN - 1) / HN;
   int bm, bn;
-  tile_coords(tiles_m, tiles_n, bm, bn);
+  tile_coords(tiles_m * tiles_n, tiles_m, tiles_n, bm, bn);
   // in scalar registers for certain (the divisions above run on the vector unit): the DMA's ranges need it
   const int row0 = __builtin_amdgcn_readfirstlane(bm * BM), col0 = __builtin_amdgcn_readfirstlane(bn * HN);
   const int kbeg = (int)blockIdx.y * P.kchunk, kend = min(P.K, kbeg + P.kchunk);

@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include "apex_amd/launch_plan.h"
+#include "apex_amd/tile_order.h"
 
 namespace apex_amd {
 namespace gemm {
@@ -137,19 +138,6 @@ __device__ __forceinline__ float dgelu_tanh(float x) {
   const float k0 = 0.7978845608028654f, k1 = 0.044715f;
   const float s = gelu_sig(x);  // (1 + tanh u) / 2;  1 - tanh^2 u = 4 s (1 - s)
   return s + 2.f * x * s * (1.f - s) * k0 * (1.f + 3.f * k1 * x * x);
-}
-
-// XCD-aware, bijective remap of the linear workgroup id, then GROUP_M-grouped tile order
-__device__ __forceinline__ void tile_coords(int nwg, int tiles_m, int tiles_n, int& bm, int& bn) {
-  const int orig = blockIdx.x;
-  const int xcd = orig % 8, q = nwg / 8, r = nwg % 8;
-  const int wgid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + orig / 8;
-  constexpr int GROUP_M = 8;
-  const int group = wgid / (GROUP_M * tiles_n);
-  const int first_m = group * GROUP_M;
-  const int gm = min(tiles_m - first_m, GROUP_M);
-  bm = first_m + (wgid % (GROUP_M * tiles_n)) % gm;
-  bn = (wgid % (GROUP_M * tiles_n)) / gm;
 }
 
 template <typename T, bool AK, bool BKM, int EPI>
