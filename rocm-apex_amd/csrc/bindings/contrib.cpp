@@ -203,8 +203,7 @@ std::vector<at::Tensor> qk_backward(const at::Tensor& gq, const at::Tensor& gk, 
 }
 
 // The autograd node lives in C++: a python one costs more host time than the kernels take at small sizes
-// (a python node that only allocates its outputs took 43 us a step where this whole operator takes 59, and
-// about 85 as a python node).
+// (16384 tokens x 32 heads x 64, forward + backward: 87 us a pass with 69 of kernels, 109 as a python node).
 struct QkNormRopeFn : torch::autograd::Function<QkNormRopeFn> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
                                                 const at::Tensor& k, const c10::optional<at::Tensor>& qw,

@@ -22,9 +22,9 @@
 // The gate and up columns of a tile are dealt so that a wave holds both for the same outputs (its
 // first BN/4 columns are rows of Wg, its last BN/4 the same rows of Wu): act(a) u is taken on the
 // accumulators, in fp32, and rounded once.
-// Measured (bf16, us of kernel): 8192 x 4096 -> 11008: gated 1230-1310 (1.13-1.2 PFLOP/s, and 0.7 GB written);
-// [da | du] 720-760; the plain products 555-660 (NT, NN, TN; 1.13-1.33 PFLOP/s, at the card's power limit:
-// 1.6 GHz).  The 128 x 64 eight-wave tiles of gemm_mfma.hip take 1296, 855 and 617-871 there.
+// Measured (bf16, us of kernel): 8192 x 4096 -> 11008: gated 1226-1310 (1.13-1.2 PFLOP/s, and 0.7 GB written);
+// [da | du] 717-760; the plain products 541-660 (NT, NN, TN; 1.13-1.36 PFLOP/s, at the card's power limit:
+// 1.3-1.7 GHz).  The 128 x 64 eight-wave tiles of gemm_mfma.hip take 1296, 855 and 617-871 there.
 //
 // The MFMAs compute the transposed tile (the n operand first), which leaves four consecutive n of one
 // row in a lane: the epilogue parks them in LDS with 8- / 16-byte writes and every global access of it
@@ -190,7 +190,8 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 // Pre-activations are kept for the backward as the upper 24 bits of their fp32 value (15 bits of
 // mantissa) in a 16- and an 8-bit plane: rounded to bf16 / fp16 they would put two more roundings of the type
 // into dx and dW1 (0.0030 instead of 0.0024 of their norm for bf16, where the result's own rounding is
-// 0.0017), for 1 % of the time.  The low bits are cut off: a NaN stays one, nothing overflows.
+// 0.0017), for 1 % of the time and 6 bytes a gate / up pair instead of 4.  The low bits are cut off, an error of
+// one sign of up to 2^-15 of a value: a NaN stays one, nothing overflows.
 __device__ __forceinline__ uint2 hi4(const float (&v)[4]) {
   return make_uint2(__builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u),
                     __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u));
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(NT, 1) ffn_gemm_kernel(const Params P) {
 // load, it kept the address unit as busy as they do (24 tokens at 2048 -> 5504 -> 2048: 32 us of kernels
 // instead of 24, now 22).  The waves' partial tiles
 // meet in LDS in a fixed order, where the block's epilogue (bias, activation, product) runs in fp32.
-// One token at 4096 -> 11008 -> 4096: 31 + 16 us, 5.8 and 5.7 TB/s of weights.
+// One token at 4096 -> 11008 -> 4096: 32-33 + 16 us, 5.5-5.7 TB/s of weights (a plain read runs at 5.8).
 // ---------------------------------------------------------------------------------------------
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <typename T>
@@ -751,7 +752,7 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // about 1.5 us for the wide tile and 1.0-1.1 for the 128-wide one, whose A fragments feed half the MFMAs.
 // Either side of the choices, us: 8192 x 1024 x 2736: 128-wide 54, wide 77, wide in two splits 70;
 // 1024 x 2736 x 8192: 128-wide in two splits 69, unsplit 108, wide in four 69; 777 x 5504 x 2048 gated: wide
-// 49, 128-wide 56; 8192 x 2736 x 1024 gradient: 128-wide 87, wide 91.
+// 49 (bf16, SiLU; fp16, GeLU 52-53), 128-wide 56; 8192 x 2736 x 1024 gradient: 128-wide 87, wide 91.
 inline Plan make_plan(const FfnArgs& g, int cus) {
   const int hn256 = g.op == kFfnGated ? 128 : 256;
   Plan best{256, 1, g.k};
@@ -819,8 +820,8 @@ bool ffn_supported(const FfnArgs& g) {
   }
 }
 
-// Up to 32 rows of a k-major x k-major product.  4096 -> 11008 -> 4096, us: 32 rows 36 + 25; 33 rows, on the
-// tiles, 49 + 28 (which 128 rows also take: 52 + 31).
+// Up to 32 rows of a k-major x k-major product.  us of kernels at 32 rows, and at 33 on the tiles (which 128 rows
+// take too, within 5): 1024 -> 2736 -> 1024 12 and 29; 2048 -> 5504 -> 2048 30 and 41; 4096 -> 11008 -> 4096 72 and 84.
 static bool ffn_few(const FfnArgs& g) { return g.m <= ffn::kFewRows && g.a_kmajor && g.b_kmajor; }
 
 FfnPlan ffn_plan(const FfnArgs& g, int cus) {

@@ -12,11 +12,11 @@
 // mean is one sum over the group's lanes.  Half-split pairs load the vectors i and i + rot/2, interleaved ones
 // 2 PV consecutive elements.  Where the rotated part or the rest is no multiple of PV pairs, its last lane
 // starts earlier: the pairs it shares with its neighbour are computed (and stored) twice and counted
-// once, which keeps every access a vector (head 80 with 34 rotated, 32768 x 16 heads bf16: 39 us forward and 77
+// once, which keeps every access a vector (head 80 with 34 rotated, 32768 x 16 heads bf16: 43-47 us forward and 75
 // backward; one pair a lane and step took 103 and 215).
 // A forward group takes two heads of its token (cosines and sines are loaded once for them, their loads are
-// in flight together), a backward group one, and the registers stay within four waves a SIMD: 51 and 81 us at
-// 32768 x 16 heads x 128 bf16, 5.2 and 4.9 TB/s (four heads and two: 56 and 90; a plain copy runs at 4.9).
+// in flight together), a backward group one, and the registers stay within four waves a SIMD: 51 and 76 us at
+// 32768 x 16 heads x 128 bf16, 5.2 and 5.3 TB/s (four heads and two: 56 and 90; a plain copy runs at 4.9).
 // Neighbouring groups take neighbouring heads, so one load instruction of a wave covers whole cache lines.
 // Blocks are dealt to q and k in proportion to their heads, so a lane's norm weights and dw sums belong to
 // one tensor for the whole kernel.
@@ -356,7 +356,8 @@ struct Plan {
 };
 
 // PV = 8 (16-byte vectors of 16-bit types) wherever the rotated part and the rest hold a lane's 8 pairs or
-// nothing (interleaved: the head does); smaller ones take one pair per lane and step.
+// nothing (interleaved: the head does); smaller ones take one pair per lane and step (32768 x 32 heads bf16, us
+// forward and backward: head 80 with 72 rotated 549 and 1257, with 80 rotated 71 and 106).
 inline Plan make_plan(const QkRopeArgs& a, int cus, bool bwd) {
   Plan p{};
   const int pairs = a.d / 2, half = a.rot / 2, rest = pairs - half;
