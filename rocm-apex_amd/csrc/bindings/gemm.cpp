@@ -360,6 +360,7 @@ void bind_gemm(pybind11::module_& root) {
   gf.def("gated_ffn", &gated_ffn);
   // (tile width, splits of K) of the six products, in order: gated, down, dW2, [da | du], dW1, dx
   gf.def("plans", [](int64_t m, int64_t k, int64_t f, int64_t n, int64_t cus) {
+    for (int64_t v : {m, k, f, n, cus}) TORCH_CHECK(v > 0 && v < (int64_t(1) << 30), "gated_ffn.plans: sizes out of range");
     struct Product { int op; bool a, b; int64_t m, n, k; };
     const Product ps[] = {{kFfnGated, true, true, m, f, k},  {kFfnPlain, true, true, m, n, f},
                           {kFfnPlain, false, false, n, f, m}, {kFfnDGated, true, false, m, f, n},

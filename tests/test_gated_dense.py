@@ -378,3 +378,9 @@ def test_gpu_wide_tiles(shape, plans, kind, bias, dtype):
 @pytest.mark.gpu
 def test_gpu_autocast_bf16():
     _autocast("cuda", torch.bfloat16)
+
+
+@pytest.mark.parametrize("shape", [(0, 64, 64, 64), (64, 0, 64, 64), (64, 64, 0, 64), (64, 64, 64, 1 << 30)])
+def test_cpu_plans_of_no_product(shape):
+    with pytest.raises(RuntimeError, match="out of range"):
+        _plans(shape, 256)
