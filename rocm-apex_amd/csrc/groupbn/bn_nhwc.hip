@@ -276,6 +276,13 @@ __device__ __forceinline__ void apply_vec(const T* __restrict__ x, const T* __re
 // per-channel coefficients are loaded once into registers instead of once per vector (they were
 // 2-5 extra 32-byte loads per 16-byte data load), and kEwU vectors are in flight per lane.
 constexpr int kEwU = 4;
+// The kEwU vectors of a trip are loaded before the first is used.  For fp32 the scheduler otherwise spends
+// few registers and waits for the vectors one by one.  us at 64 x 56 x 56 x 256 with and without: backward behind a
+// ReLU 103 and 184, the two-input forward 107 and 164; where it keeps the order itself, 3 % slower with it (105, 108).
+template <typename T>
+__device__ __forceinline__ void loads_first() {
+  if constexpr (sizeof(T) == 4) __builtin_amdgcn_sched_barrier(0);
+}
 
 template <typename T, bool HAS_Z, bool RELU, bool MASKOUT>
 __global__ void __launch_bounds__(256) apply_kernel(const T* __restrict__ x, const T* __restrict__ z,
@@ -359,6 +366,7 @@ __global__ void __launch_bounds__(256) apply_dual_kernel(const T* __restrict__ x
         Vec8<T>::load(v[u], x + (i + u * stride) * 8);
         Vec8<T>::load(w[u], z + (i + u * stride) * 8);
       }
+      loads_first<T>();
 #pragma unroll
       for (int u = 0; u < kEwU; ++u) apply_dual_vec<T, MASKOUT>(y, mask, i + u * stride, v[u], w[u], sx, hx, sz, hz);
     }
@@ -624,6 +632,7 @@ __global__ void __launch_bounds__(256) bwd_apply(const T* __restrict__ dy, const
         Vec8<T>::load(v[u], x + (i + u * stride) * 8);
         if constexpr (MASK && HAS_Z) Vec8<T>::load(zu[u], z + (i + u * stride) * 8);
       }
+      if constexpr (MASK && !HAS_Z) loads_first<T>();
 #pragma unroll
       for (int u = 0; u < kEwU; ++u)
         bwd_apply_vec<T, HAS_Z, MASK>(dx, i + u * stride, g[u], v[u], zu[u], A, B, K, sc, sh);
